@@ -411,6 +411,83 @@ int tops_qconv_levels_shape(const int x_shape[4], const int kernel[2], const Con
 int tops_dynamic_quantize_range(const Tensor* x, Tensor* range);
 int tops_dynamic_quantize_apply(const Tensor* x, const Tensor* range, Tensor* y, Tensor* y_scale, Tensor* y_zp);
 
+/* ---- attention with cached keys and values (no counterpart in the reference: its graphs run MatMul, Softmax and
+   element-wise nodes for this, nn/Operators.py:1361-1432, 671-704) ------------------------------------------------
+
+   Three operators of a decoder that run one after the other.  Activations are float16, bfloat16 or float32 (one type per
+   call), sums and softmax statistics are float32, every result is rounded once.  Tensors are dense; a cache is
+   [pages, page_size, kv_heads, dim].  Index tensors live in device memory and are not read by the host: an index that
+   points outside its table is never followed -- the row it belongs to is zero-filled (or, for a page, reads as zero keys and values; for
+   a slot, is not stored) and the next tops_sync or download reports TOPS_ERR_INVALID.  No call allocates device memory or
+   keeps state, so captured sequences and other streams may run the same operators at the same time.
+   Return TOPS_OK or the recorded error; a rejected call zero-fills its outputs and leaves caches and operands that an output shares memory with as they
+   were. */
+
+/* RMS norm of every query and key head, then the rotary position embedding, then (optionally) the append to a paged cache,
+   in one pass:   n = x / sqrt(mean(x^2) + epsilon) * weight
+                  rotated pairs (a, b) of n -> (a * cos - b * sin, a * sin + b * cos), the rest of the head is passed on
+   Pairs are (i, i + rotary_dim / 2), or with `interleaved` (2i, 2i + 1); rotary_dim is twice the tables' second extent. */
+typedef struct QKNormRotaryCall {
+    const Tensor* q;            /* [..., S, H, D]; heads_first: [B, H, S, D]; packed: [..., S, H + 2 * packed_kv_heads, D] */
+    const Tensor* k;            /* the same with the key heads, or NULL (packed, or queries only) */
+    const Tensor* v;            /* the shape of k; only read for the cache, which it is copied to */
+    int packed_kv_heads;        /* > 0: k and v are NULL and follow the queries inside q's heads axis */
+    int heads_first;            /* q, k, v, q_out and k_out are [B, H, S, D] (not with packed) */
+    const Tensor* q_weight;     /* [D] of the activations' type or float32; NULL: queries are not normalised */
+    const Tensor* k_weight;     /* the same for keys */
+    float epsilon;
+    const Tensor* cos_table;    /* float32 [P, rotary_dim / 2]; both NULL: no rotation */
+    const Tensor* sin_table;
+    const Tensor* positions;    /* int32 or int64, one per token (B * S): row of the tables */
+    int interleaved;
+    Tensor* q_out;              /* [..., S, H, D]; may be q itself (not with packed) */
+    Tensor* k_out;              /* the key heads' counterpart, may be k itself; NULL when only the cache is wanted */
+    Tensor* key_cache;          /* [pages, page_size, kv_heads, D]; both or neither */
+    Tensor* value_cache;
+    const Tensor* slots;        /* int32 or int64, one per token: page * page_size + offset; negative: the token is not stored.
+                                   Two tokens of one call that name the same slot leave either one's row there. */
+} QKNormRotaryCall;
+int tops_qk_norm_rotary_forward(const QKNormRotaryCall* call);
+
+/* A ragged batch of new tokens attends over the paged cache that already holds their keys and values:
+     y[t, h] = softmax_j(scale * q[t, h] . K[j, h / (H / kv_heads)]) V[j, ...]
+   Sequence b owns the rows query_start[b] .. query_start[b + 1] - 1 of q and y and kv_length[b] keys, its new tokens' own
+   included: the i-th of n new tokens stands at position p = kv_length[b] - n + i and sees the keys j <= p, with a window
+   also only j > p - window.  A token that sees no key (p < 0) gets zeros; rows of y in front of query_start[0] and behind
+   query_start[B] are left as they are.  One new token per sequence and whole prompts are both served; float16 / bfloat16 heads of
+   up to 256 (a multiple of 8) run on tensor cores, the rest in float32 arithmetic.  Keys and values behind kv_length may hold
+   anything.  The tables have to be consistent: 0 <= query_start[b] <= query_start[b + 1] <= rows of q (rows outside are not
+   touched), kv_length[b] <= table width * page_size (more is cut to that). */
+typedef struct PagedAttentionCall {
+    const Tensor* q;            /* [T, H, D] */
+    const Tensor* key_cache;    /* [pages, page_size, kv_heads, D], H a multiple of kv_heads */
+    const Tensor* value_cache;
+    const Tensor* page_table;   /* int32 [B, width]: the pages of each sequence in order; entries behind its length are not read */
+    const Tensor* query_start;  /* int32 [B + 1] */
+    const Tensor* kv_length;    /* int32 [B] */
+    float scale;                /* finite */
+    int window;                 /* 0: none */
+    Tensor* y;                  /* [T, H, D], not q's memory */
+} PagedAttentionCall;
+int tops_paged_attention_forward(const PagedAttentionCall* call);
+
+/* Queries attend to an encoder's states of another length (not causal):
+     y[b, i, h] = softmax_j(scale * q[b, i, h] . k[b, j, h / (H / kv_heads)] + mask[b, j]) v[b, j, ...]
+   key_length and mask may be given together.  Excluded keys: j >= key_length[b]; a uint8 / int8 mask of 0; a float mask of -Inf or of its
+   type's lowest finite value.  They do not enter the result whatever k and v hold there (NaN included); a row of the batch
+   with no key left gives zeros. */
+typedef struct CrossAttentionCall {
+    const Tensor* q;            /* [B, Lq, H, D], heads_first: [B, H, Lq, D] */
+    const Tensor* k;            /* [B, Lk, kv_heads, D], heads_first: [B, kv_heads, Lk, D] */
+    const Tensor* v;            /* the shape of k */
+    const Tensor* key_length;   /* int32 [B] or NULL */
+    const Tensor* mask;         /* B * Lk elements ([B, Lk], [B, 1, 1, Lk]), uint8 / int8 (non-zero: attend), float32 or q's type (added); or NULL */
+    float scale;                /* finite */
+    int heads_first;
+    Tensor* y;                  /* the shape of q, not the memory of q, k or v */
+} CrossAttentionCall;
+int tops_cross_attention_forward(const CrossAttentionCall* call);
+
 /* Device-side exhaustive codec self-check: encodes every float32 bit pattern with the fast
    (hardware-convert) encoder and with the bit-level restatement of the reference encoder and
    returns the number of disagreements (NaN inputs excluded), or -1 on error. */

@@ -44,6 +44,28 @@ class CQConvCall(ctypes.Structure):
                 ("x_channels_last", ctypes.c_int), ("y_channels_last", ctypes.c_int), ("residual_channels_last", ctypes.c_int)]
 
 
+class CQKNormRotaryCall(ctypes.Structure):
+    """QKNormRotaryCall of tensor_ops_b200.h."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("packed_kv_heads", ctypes.c_int),
+                ("heads_first", ctypes.c_int), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("epsilon", ctypes.c_float),
+                ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("interleaved", ctypes.c_int),
+                ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("key_cache", ctypes.c_void_p), ("value_cache", ctypes.c_void_p),
+                ("slots", ctypes.c_void_p)]
+
+
+class CPagedAttentionCall(ctypes.Structure):
+    """PagedAttentionCall of tensor_ops_b200.h."""
+    _fields_ = [("q", ctypes.c_void_p), ("key_cache", ctypes.c_void_p), ("value_cache", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("query_start", ctypes.c_void_p), ("kv_length", ctypes.c_void_p), ("scale", ctypes.c_float), ("window", ctypes.c_int),
+                ("y", ctypes.c_void_p)]
+
+
+class CCrossAttentionCall(ctypes.Structure):
+    """CrossAttentionCall of tensor_ops_b200.h."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("key_length", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+                ("scale", ctypes.c_float), ("heads_first", ctypes.c_int), ("y", ctypes.c_void_p)]
+
+
 class CPoolParams(ctypes.Structure):
     _fields_ = [("pads", ctypes.POINTER(ctypes.c_int)), ("strides", ctypes.POINTER(ctypes.c_int)),
                 ("dilations", ctypes.POINTER(ctypes.c_int)), ("kernel_shape", ctypes.POINTER(ctypes.c_int))]
@@ -158,6 +180,9 @@ SIGNATURES = {
     "tops_qconv_forward": (_I, [ctypes.POINTER(CQConvCall)]),
     "tops_qconv_levels_shape": (_I, [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int), ctypes.POINTER(CConvParams),
                                      ctypes.POINTER(ctypes.c_int)]),
+    "tops_qk_norm_rotary_forward": (_I, [ctypes.POINTER(CQKNormRotaryCall)]),
+    "tops_paged_attention_forward": (_I, [ctypes.POINTER(CPagedAttentionCall)]),
+    "tops_cross_attention_forward": (_I, [ctypes.POINTER(CCrossAttentionCall)]),
     "tops_selftest_encoder": (ctypes.c_longlong, [_I]),
     "tops_tensor_core_launches": (ctypes.c_longlong, []),
     "tops_selftest_cos": (ctypes.c_longlong, []),

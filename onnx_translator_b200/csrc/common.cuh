@@ -40,6 +40,8 @@ const double* cos_lut_device();           // uploads on first use
 int*         device_status_word();        // device pointer to the host-visible status word (may be null)
 int*         device_status_word_if_created();   // as above, but never allocates (null until first created)
 void         poll_device_status();        // host: turn a raised status word into an error
+constexpr int kStatusBadIndex = 2;        // status word: an index read from device memory was outside its table (any other value: a wait expired)
+int          tensor_device(const Tensor* t);   // device index recorded when the tensor was made; -1 if not one of this library's
 // Opt-in for more than 48 KB of dynamic shared memory.  The attribute belongs to the (kernel, device) pair, so
 // it is recorded per device: the first launch of `kernel` on each device sets it, with that device current.
 bool         ensure_dynamic_smem(const void* kernel, size_t bytes);

@@ -1,0 +1,289 @@
+// RMS norm of every query and key head, the rotary position embedding, and the append of keys and values to a paged cache, in
+// one pass over the projection.
+//
+//   n = x * rsqrt(mean(x^2) + epsilon) * weight;   (a, b) -> (a cos - b sin, a sin + b cos)
+//
+// Each element is read once and written once (HBM bound); norms and rotations are float32, rounded once when stored.
+#include "attention_common.cuh"
+#include "call_checks.cuh"
+
+#include <cmath>
+
+namespace tops {
+
+struct HeadsView {                           // strides in elements
+    const void* in = nullptr;
+    void* out = nullptr;                     // null: not written here
+    void* cache = nullptr;                   // null: not appended
+    const void* weight = nullptr;            // null: no norm
+    int weight_f32 = 0;
+    int heads = 0;
+    int rotate = 0;
+    long long in_batch = 0, in_token = 0, in_head = 0;
+    long long out_batch = 0, out_token = 0, out_head = 0;
+};
+
+struct NormRotaryProblem {
+    HeadsView part[3];                       // queries, keys, values
+    int blocks[3] = {0, 0, 0};               // head blocks of each part
+    int tokens = 0, seq = 1;                 // tokens in all; per batch row (heads_first)
+    FastDiv seq_div, block_div;
+    int dim = 0, half = 0;                   // half = rotary_dim / 2
+    int interleaved = 0;
+    float epsilon = 0.0f, inv_dim = 0.0f;
+    const float* cos_table = nullptr;
+    const float* sin_table = nullptr;
+    int table_rows = 0;
+    const void* positions = nullptr;
+    int positions_64 = 0;
+    const void* slots = nullptr;
+    int slots_64 = 0;
+    long long cache_rows = 0;
+    int cache_heads = 0;
+    int* status = nullptr;
+};
+
+__device__ __forceinline__ long long read_index(const void* p, int is64, int i) {
+    return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
+}
+
+// Where a token's rows go: its table row (-1: none) and cache slot (-1: not stored).
+struct TokenPlace { int batch, in_row, table_row; long long slot; bool bad_position; };
+
+__device__ __forceinline__ TokenPlace place_token(const NormRotaryProblem& p, int token, bool positioned, bool append) {
+    TokenPlace at;
+    at.batch = (int)p.seq_div.div((uint32_t)token);
+    at.in_row = token - at.batch * p.seq;
+    at.table_row = -1;
+    at.slot = -1;
+    at.bad_position = false;
+    if (positioned) {
+        const long long pos = read_index(p.positions, p.positions_64, token);
+        if (pos >= 0 && pos < p.table_rows) at.table_row = (int)pos;
+        else { at.bad_position = true; if (p.status) atomicExch(p.status, kStatusBadIndex); }
+    }
+    if (append) {
+        at.slot = read_index(p.slots, p.slots_64, token);
+        if (at.slot >= p.cache_rows) { at.slot = -1; if (p.status) atomicExch(p.status, kStatusBadIndex); }
+    }
+    return at;
+}
+
+template <typename T> __device__ __forceinline__ float read_weight(const HeadsView& h, int d) {
+    return h.weight_f32 ? reinterpret_cast<const float*>(h.weight)[d] : to_float(reinterpret_cast<const T*>(h.weight)[d]);
+}
+
+// General form: a warp per (token, head), elements strided over the lanes, the normalised head staged in shared memory so that
+// any pairing of elements can be read back.  Takes every head size, alignment and rotary extent.
+template <typename T>
+__global__ void __launch_bounds__(128) norm_rotary_general(const __grid_constant__ NormRotaryProblem p) {
+    extern __shared__ float staged[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* mine = staged + warp * p.dim;
+    const int per_token = p.part[0].heads + p.part[1].heads + p.part[2].heads;
+    const long long items = (long long)p.tokens * per_token;
+    for (long long item = (long long)blockIdx.x * 4 + warp; item < items; item += (long long)gridDim.x * 4) {
+        const int token = (int)(item / per_token);
+        int head = (int)(item - (long long)token * per_token), which = 0;
+        while (head >= p.part[which].heads) head -= p.part[which++].heads;
+        const HeadsView& h = p.part[which];
+        const TokenPlace at = place_token(p, token, p.positions != nullptr, h.cache != nullptr);
+        const T* in = reinterpret_cast<const T*>(h.in) + at.batch * h.in_batch + at.in_row * h.in_token + head * h.in_head;
+        float sum = 0.0f;
+        for (int d = lane; d < p.dim; d += 32) {
+            const float x = to_float(in[d]);
+            mine[d] = x;
+            sum = __fmaf_rn(x, x, sum);
+        }
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        const float factor = rsqrtf(__fmaf_rn(sum, p.inv_dim, p.epsilon));
+        __syncwarp();
+        if (h.weight) for (int d = lane; d < p.dim; d += 32) mine[d] = mine[d] * factor * read_weight<T>(h, d);
+        __syncwarp();
+        T* out = h.out ? reinterpret_cast<T*>(h.out) + at.batch * h.out_batch + at.in_row * h.out_token + head * h.out_head : nullptr;
+        T* cache = h.cache && at.slot >= 0 && !at.bad_position ? reinterpret_cast<T*>(h.cache) + (at.slot * p.cache_heads + head) * p.dim : nullptr;
+        for (int d = lane; d < p.dim; d += 32) {
+            float y = mine[d];
+            if (h.rotate && d < 2 * p.half && at.table_row >= 0) {
+                const bool second = p.interleaved ? (d & 1) : d >= p.half;
+                const int pair = p.interleaved ? d >> 1 : (second ? d - p.half : d);
+                const float other = mine[p.interleaved ? d ^ 1 : (second ? d - p.half : d + p.half)];
+                const float c = p.cos_table[(long long)at.table_row * p.half + pair], s = p.sin_table[(long long)at.table_row * p.half + pair];
+                y = second ? __fmaf_rn(other, s, y * c) : __fmaf_rn(y, c, -(other * s));
+            }
+            if (at.bad_position) y = 0.0f;
+            if (out) out[d] = from_float<T>(y);
+            if (cache) cache[d] = from_float<T>(y);
+        }
+        __syncwarp();
+    }
+}
+
+template <typename T> static bool launch_general(const NormRotaryProblem& p) {
+    DeviceState* st = acquire_device();
+    if (!st) return false;
+    const long long items = (long long)p.tokens * (p.part[0].heads + p.part[1].heads + p.part[2].heads);
+    const int blocks = grid_for((size_t)items, 4, st->sm_count, 16);
+    norm_rotary_general<T><<<blocks, 128, 4 * sizeof(float) * (size_t)p.dim, current_stream()>>>(p);
+    return TOPS_CHECK_LAUNCH("norm_rotary_general");
+}
+
+static bool run_norm_rotary(const NormRotaryProblem& p, int dtype) {
+    switch (dtype) {
+        case DTYPE_FLOAT16:  return launch_general<__half>(p);
+        case DTYPE_BFLOAT16: return launch_general<__nv_bfloat16>(p);
+        default:             return launch_general<float>(p);
+    }
+}
+
+// Strides of a dense [..., S, H, D] or, heads_first, [B, H, S, D] tensor with `heads_in_memory` heads.
+static void strides_of(long long& batch, long long& token, long long& head, bool heads_first, long long seq, long long heads_in_memory, long long dim) {
+    batch = seq * heads_in_memory * dim;
+    token = heads_first ? dim : heads_in_memory * dim;
+    head = heads_first ? seq * dim : dim;
+}
+
+}  // namespace tops
+
+using namespace tops;
+
+TOPS_API int tops_qk_norm_rotary_forward(const QKNormRotaryCall* call) {
+    const char* name = "tops_qk_norm_rotary_forward";
+    if (!call) return call_fail(name, TOPS_ERR_INVALID, "null call", {});
+    const QKNormRotaryCall& c = *call;
+    OutputList outs;
+    for (const Tensor* t : {(const Tensor*)c.q_out, (const Tensor*)c.k_out}) if (t) outs.tensors[outs.count++] = t;
+    outs.outputs = outs.count;
+    for (const Tensor* t : {c.q, c.k, c.v, c.q_weight, c.k_weight, c.cos_table, c.sin_table, c.positions, (const Tensor*)c.key_cache, (const Tensor*)c.value_cache, c.slots})
+        outs.tensors[outs.count++] = t;
+    auto fail = [&](int code, const char* what) { return call_fail(name, code, what, outs); };
+    for (int i = 0; i < outs.count; i++)
+        if (outs.tensors[i] && !outs.tensors[i]->data) return fail(TOPS_ERR_INVALID, "a tensor without data");
+    if (!c.q || !c.q_out) return fail(TOPS_ERR_INVALID, "q and q_out are required");
+    const bool packed = c.packed_kv_heads > 0, first = c.heads_first != 0, cached = c.key_cache != nullptr;
+    if (c.packed_kv_heads < 0 || (packed && (c.k || c.v || first))) return fail(TOPS_ERR_INVALID, "packed keys and values come inside q: k and v NULL, not heads_first");
+    if (c.q->ndim < 2 || (first && c.q->ndim != 4)) return fail(TOPS_ERR_INVALID, "q is [..., tokens, heads, dim] or, heads_first, [batch, heads, tokens, dim]");
+    const int nd = c.q->ndim, dim = c.q->shape[nd - 1], heads_at = first ? 1 : nd - 2;
+    const int heads = c.q->shape[heads_at] - (packed ? 2 * c.packed_kv_heads : 0);
+    if (dim < 1 || dim > 1024) return fail(TOPS_ERR_UNSUPPORTED, "heads of 1 to 1024 elements");
+    if (heads < 1) return fail(TOPS_ERR_INVALID, "no query heads");
+    const int dt = c.q->dtype;
+    if (dt != DTYPE_FLOAT16 && dt != DTYPE_BFLOAT16 && dt != DTYPE_FLOAT32) return fail(TOPS_ERR_UNSUPPORTED, "float16, bfloat16 or float32");
+    const size_t token_count = c.q->size / ((size_t)c.q->shape[heads_at] * (size_t)dim);
+    if (c.q->size >= 0x7FFFFFFFull * 16 || token_count >= 0x7FFFFFFFull / 64) return fail(TOPS_ERR_UNSUPPORTED, "fewer than 2^25 tokens");
+    // shapes of the outputs: q's with its own heads
+    auto shaped = [&](const Tensor* t, int want_heads) {
+        if (t->ndim != nd || t->dtype != dt) return false;
+        for (int i = 0; i < nd; i++) if (t->shape[i] != (i == heads_at ? want_heads : c.q->shape[i])) return false;
+        return true;
+    };
+    if (!shaped(c.q_out, heads)) return fail(TOPS_ERR_INVALID, "q_out has q's shape (packed: with the query heads alone) and type");
+    int kv_heads = packed ? c.packed_kv_heads : 0;
+    if (c.k) {
+        if (c.k->ndim != nd) return fail(TOPS_ERR_INVALID, "k has q's rank");
+        kv_heads = c.k->shape[heads_at];
+        if (kv_heads < 1 || !shaped(c.k, kv_heads)) return fail(TOPS_ERR_INVALID, "k has q's shape but for the heads, and its type");
+    }
+    const bool keys = packed || c.k;
+    if (c.v && (!c.k || !shaped(c.v, kv_heads))) return fail(TOPS_ERR_INVALID, "v has k's shape and type");
+    if (c.k_out && (!keys || !shaped(c.k_out, kv_heads))) return fail(TOPS_ERR_INVALID, "k_out has the key heads' shape and type");
+    if (keys && !c.k_out && !cached) return fail(TOPS_ERR_INVALID, "keys need k_out or a cache to go to");
+    if (cached != (c.value_cache != nullptr) || cached != (c.slots != nullptr) || (cached && (!keys || (!packed && !c.v))))
+        return fail(TOPS_ERR_INVALID, "key_cache, value_cache and slots come together, with keys and values to store");
+    if (!cached && c.v) return fail(TOPS_ERR_INVALID, "v is only read for a cache");
+    if (cached) {
+        const Tensor* kc = c.key_cache;
+        if (kc->ndim != 4 || !same_shape(kc, c.value_cache) || kc->dtype != dt || c.value_cache->dtype != dt || kc->shape[2] != kv_heads || kc->shape[3] != dim)
+            return fail(TOPS_ERR_INVALID, "key_cache and value_cache are [pages, page_size, kv_heads, dim] of q's type");
+        if ((c.slots->dtype != DTYPE_INT32 && c.slots->dtype != DTYPE_INT64) || c.slots->size != token_count)
+            return fail(TOPS_ERR_INVALID, "slots is int32 or int64 with one entry per token");
+    }
+    for (const Tensor* w : {c.q_weight, c.k_weight})
+        if (w && (w->size != (size_t)dim || (w->dtype != dt && w->dtype != DTYPE_FLOAT32))) return fail(TOPS_ERR_INVALID, "weights have dim elements of q's type or float32");
+    if (c.k_weight && !keys) return fail(TOPS_ERR_INVALID, "k_weight without keys");
+    if ((c.q_weight || c.k_weight) && !(std::isfinite(c.epsilon) && c.epsilon >= 0.0f)) return fail(TOPS_ERR_INVALID, "epsilon is finite and not negative");
+    const bool rotate = c.cos_table != nullptr;
+    if (rotate != (c.sin_table != nullptr) || rotate != (c.positions != nullptr)) return fail(TOPS_ERR_INVALID, "cos_table, sin_table and positions come together");
+    if (rotate) {
+        if (c.cos_table->ndim != 2 || !same_shape(c.cos_table, c.sin_table) || c.cos_table->dtype != DTYPE_FLOAT32 || c.sin_table->dtype != DTYPE_FLOAT32 ||
+            c.cos_table->shape[1] < 1 || 2 * (long long)c.cos_table->shape[1] > dim)
+            return fail(TOPS_ERR_INVALID, "the tables are float32 [positions, rotary_dim / 2] with rotary_dim at most dim");
+        if ((c.positions->dtype != DTYPE_INT32 && c.positions->dtype != DTYPE_INT64) || c.positions->size != token_count)
+            return fail(TOPS_ERR_INVALID, "positions is int32 or int64 with one entry per token");
+    }
+    // an output may be its own operand, element for element, and nothing else
+    for (int i = 0; i < outs.outputs; i++)
+        for (int j = i + 1; j < outs.count; j++) {
+            const Tensor *o = outs.tensors[i], *t = outs.tensors[j];
+            const bool itself = !packed && ((o == c.q_out && t == c.q) || (o == c.k_out && t == c.k)) && o->data == t->data;
+            if (!itself && overlap(o, t)) return fail(TOPS_ERR_INVALID, "an output shares memory with another tensor of the call");
+        }
+    if (cached && overlap(c.key_cache, c.value_cache)) return fail(TOPS_ERR_INVALID, "the two caches share memory");
+    if (cached)
+        for (const Tensor* cache : {c.key_cache, c.value_cache})
+            for (int j = outs.outputs; j < outs.count; j++)
+                if (outs.tensors[j] != c.key_cache && outs.tensors[j] != c.value_cache && overlap(cache, outs.tensors[j])) return fail(TOPS_ERR_INVALID, "a cache shares memory with another tensor of the call");
+    for (int i = 0; i < outs.count; i++)
+        if (!on_current_device({outs.tensors[i]})) return call_fail(name, TOPS_ERR_INVALID, "a tensor belongs to another device than the current one", {});
+    if (!acquire_device()) return tops_last_error();
+    if (token_count == 0) return TOPS_OK;
+
+    NormRotaryProblem p;
+    const long long size = dtype_bytes(dt);
+    p.tokens = (int)token_count;
+    p.seq = first ? c.q->shape[2] : p.tokens;
+    p.seq_div.set((uint32_t)p.seq);
+    p.dim = dim;
+    p.half = rotate ? c.cos_table->shape[1] : 0;
+    p.interleaved = c.interleaved != 0;
+    p.epsilon = c.epsilon;
+    p.inv_dim = 1.0f / (float)dim;
+    if (rotate) {
+        p.cos_table = reinterpret_cast<const float*>(c.cos_table->data);
+        p.sin_table = reinterpret_cast<const float*>(c.sin_table->data);
+        p.table_rows = c.cos_table->shape[0];
+        p.positions = c.positions->data;
+        p.positions_64 = c.positions->dtype == DTYPE_INT64;
+    }
+    if (cached) {
+        p.slots = c.slots->data;
+        p.slots_64 = c.slots->dtype == DTYPE_INT64;
+        p.cache_rows = (long long)c.key_cache->shape[0] * c.key_cache->shape[1];
+        p.cache_heads = kv_heads;
+    }
+    p.status = device_status_word();
+    HeadsView& q = p.part[0];
+    q.in = c.q->data;
+    q.out = c.q_out->data;
+    q.weight = c.q_weight ? c.q_weight->data : nullptr;
+    q.weight_f32 = c.q_weight && c.q_weight->dtype == DTYPE_FLOAT32;
+    q.heads = heads;
+    q.rotate = rotate;
+    strides_of(q.in_batch, q.in_token, q.in_head, first, p.seq, c.q->shape[heads_at], dim);
+    strides_of(q.out_batch, q.out_token, q.out_head, first, p.seq, heads, dim);
+    if (keys) {
+        HeadsView& k = p.part[1];
+        k = q;
+        k.in = packed ? (const char*)c.q->data + (long long)heads * dim * size : (const char*)c.k->data;
+        k.out = c.k_out ? c.k_out->data : nullptr;
+        k.cache = cached ? c.key_cache->data : nullptr;
+        k.weight = c.k_weight ? c.k_weight->data : nullptr;
+        k.weight_f32 = c.k_weight && c.k_weight->dtype == DTYPE_FLOAT32;
+        k.heads = kv_heads;
+        if (!packed) strides_of(k.in_batch, k.in_token, k.in_head, first, p.seq, kv_heads, dim);
+        strides_of(k.out_batch, k.out_token, k.out_head, first, p.seq, kv_heads, dim);
+        if (cached) {
+            HeadsView& v = p.part[2];
+            v = k;
+            v.in = packed ? (const char*)k.in + (long long)kv_heads * dim * size : (const char*)c.v->data;
+            v.out = nullptr;
+            v.cache = c.value_cache->data;
+            v.weight = nullptr;
+            v.rotate = 0;
+        }
+    }
+    if (!run_norm_rotary(p, dt)) return tops_last_error();
+    finish_op();
+    return TOPS_OK;
+}

@@ -216,6 +216,12 @@ static void release(TensorImpl* impl) {
     }
 }
 
+// The device a tensor of this library was made on; -1 for headers that it did not make.
+int tensor_device(const Tensor* t) {
+    const TensorImpl* impl = impl_of(t);
+    return impl ? impl->device : -1;
+}
+
 void zero_fill(Tensor* t) {
     if (!t || !t->data || t->size == 0) return;
     if (!acquire_device()) return;
@@ -592,8 +598,12 @@ int* device_status_word_if_created() {
 
 void poll_device_status() {
     if (g_status_host && *(volatile int*)g_status_host) {
+        const int status = *(volatile int*)g_status_host;
         *(volatile int*)g_status_host = 0;
-        set_error(TOPS_ERR_DEVICE_TIMEOUT, "a bounded device-side wait expired inside a tensor-core kernel");
+        if (status == kStatusBadIndex)
+            set_error(TOPS_ERR_INVALID, "an index in device memory (position, slot, page or sequence bound) pointed outside its table; it was not followed");
+        else
+            set_error(TOPS_ERR_DEVICE_TIMEOUT, "a bounded device-side wait expired inside a tensor-core kernel");
     }
 }
 }  // namespace tops

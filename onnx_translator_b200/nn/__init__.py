@@ -179,3 +179,4 @@ def synchronize() -> None:
 
 from .graph import Graph, qdq_resnet50, small_cnn  # noqa: E402  (the graph runner builds on the classes above)
 from .plan import GraphPlan  # noqa: E402
+from .attention_ops import CrossAttention, PagedAttention, QKNormRotary  # noqa: E402

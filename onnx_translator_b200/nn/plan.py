@@ -25,10 +25,12 @@ import ctypes
 from typing import List, Sequence
 
 from .. import capi
-from ..capi import CQConvCall, TensorP
+from ..capi import CCrossAttentionCall, CPagedAttentionCall, CQConvCall, CQKNormRotaryCall, TensorP
 
-# struct members of QConvCall that hold tensor handles
-_QCONV_TENSOR_FIELDS = ("x", "x_scale", "x_zero", "w_codes", "w_scale", "bias", "residual", "y", "y_levels", "next_scale", "next_zero")
+# members that hold tensor handles, of the structs that operators take
+_TENSOR_FIELDS = {CQConvCall: ("x", "x_scale", "x_zero", "w_codes", "w_scale", "bias", "residual", "y", "y_levels", "next_scale", "next_zero")}
+_TENSOR_FIELDS.update({struct: tuple(name for name, kind in struct._fields_ if kind is ctypes.c_void_p)
+                       for struct in (CQKNormRotaryCall, CPagedAttentionCall, CCrossAttentionCall)})
 # calls that are part of the computation although their names do not end in _forward
 _ALSO_RECORDED = {"tops_dynamic_quantize_range", "tops_dynamic_quantize_apply"}
 # calls that move data to the host or wait for the device: a forward pass that needs them cannot be replayed blindly
@@ -50,13 +52,13 @@ class _Recorder:
             self._lib.tops_retain(handle)
             self.held.append(handle)
 
-    def _hold_arguments(self, name, args) -> None:
+    def _hold_arguments(self, args) -> None:
         for a in args:
             if isinstance(a, TensorP):
                 self._hold(a)
-            elif name == "tops_qconv_forward" and isinstance(getattr(a, "_obj", None), CQConvCall):
+            elif type(getattr(a, "_obj", None)) in _TENSOR_FIELDS:
                 call = a._obj
-                for field in _QCONV_TENSOR_FIELDS:
+                for field in _TENSOR_FIELDS[type(call)]:
                     ptr = getattr(call, field)
                     if ptr:
                         self._hold(ctypes.cast(ptr, TensorP))
@@ -74,7 +76,7 @@ class _Recorder:
             return fn
 
         def recorded(*args):
-            self._hold_arguments(name, args)
+            self._hold_arguments(args)
             self.calls.append((fn, args))
             return fn(*args)
         return recorded
