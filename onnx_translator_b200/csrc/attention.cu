@@ -42,7 +42,14 @@ bool launch_attention(const void* kernel, const AttentionProblem& p, int rows_pe
     return check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), name);
 }
 
+// 16-bit rows of 16-byte pieces on 16-byte boundaries can be copied asynchronously and read as matrix fragments.
+static bool whole_pieces(const AttentionProblem& p) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | reinterpret_cast<uintptr_t>(p.y);
+    return p.dtype != DTYPE_FLOAT32 && p.dim % 8 == 0 && (bits & 15) == 0;
+}
+
 static bool run_attention(const AttentionProblem& p) {
+    if (whole_pieces(p)) return attention_rows(p);
     return attention_fma(p);
 }
 

@@ -77,9 +77,10 @@ __device__ __forceinline__ bool locate_tile(const AttentionProblem& p, int index
         bool found = false;
         for (int base = 0; base < p.batch; base += 32) {
             const int b = base + lane;
-            int start = 0, end = 0;
+            int start = 0, end = 0, length = 0;
             if (b < p.batch) {
                 const int s = p.query_start[b], e = p.query_start[b + 1];
+                length = p.kv_length[b];                     // fetched along with the bounds: one round trip less
                 start = min(max(s, 0), p.queries);
                 end = min(max(e, start), p.queries);
                 if (start != s || end != e) report_bad_index(p);
@@ -95,13 +96,14 @@ __device__ __forceinline__ bool locate_tile(const AttentionProblem& p, int index
                 t.token0 = __shfl_sync(~0u, start, at);
                 tokens = __shfl_sync(~0u, end, at) - t.token0;
                 t.row0 = (index - before - __shfl_sync(~0u, sum - tiles, at)) * rows_per_tile;
+                t.length = __shfl_sync(~0u, length, at);
                 found = true;
                 break;
             }
             before += __shfl_sync(~0u, sum, 31);
         }
         if (!found) return false;
-        const int length = p.kv_length[t.seq];
+        const int length = t.length;
         t.length = min(max(length, 0), p.keys);
         if (length != t.length) report_bad_index(p);
         t.first_position = t.length - tokens;
@@ -185,6 +187,30 @@ template <typename T> __device__ __forceinline__ void store4(T* to, const float 
     } else {
         for (int i = 0; i < left && i < 4; i++) to[i] = from_float<T>(x[i]);
     }
+}
+
+// ---- the warp-level building blocks of the 16-bit kernels ---------------------------------------------------------------
+// 16 bytes global -> shared without a register, zeros when `bytes` is 0 (nothing is read then).
+__device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void load_matrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_matrix4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// c[16 x 8] += a[16 x 16] b[16 x 8], float32 accumulators.
+template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // ---- clusters --------------------------------------------------------------------------------------------------------

@@ -129,11 +129,168 @@ template <typename T> static bool launch_general(const NormRotaryProblem& p) {
     return TOPS_CHECK_LAUNCH("norm_rotary_general");
 }
 
+// Vector form: dim a multiple of 8 up to 256, 16-byte aligned rows.  LPH lanes hold a head, eight neighbouring elements each, and
+// work through HB heads of one token: all HB loads are in flight before the first use, and the token's cosines and sines are
+// read once for the HB heads.  With pairs (i, i + half) the partner elements sit in another lane of the head (a shuffle), with
+// interleaved pairs in the same lane.
+template <typename T> __device__ __forceinline__ void load8(const T* from, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(from);
+        const T* t = reinterpret_cast<const T*>(&a);
+        #pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_float(t[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+    }
+}
+
+constexpr int kNormThreads = 128;
+
+template <typename T, int LPH, int HB, bool INTERLEAVED>
+__global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_constant__ NormRotaryProblem p, const uint32_t items) {
+    constexpr int PER_WARP = 32 / LPH;
+    const int lane = threadIdx.x & 31, in_head = lane % LPH, group = lane / LPH;
+    const uint32_t warp = blockIdx.x * (kNormThreads / 32) + (threadIdx.x >> 5), warps = gridDim.x * (kNormThreads / 32);
+    const int d = in_head * 8;
+    const bool mine = d < p.dim;
+    const int half = p.half;
+    // the lane that holds the other halves of this lane's pairs
+    const bool second = !INTERLEAVED && d >= half;
+    const int partner = (lane - in_head) + (d < 2 * half ? (second ? d - half : d + half) / 8 : in_head);
+    for (uint32_t base = warp * PER_WARP; base < items; base += warps * PER_WARP) {
+        const uint32_t item = base + group;
+        const bool there = item < items;
+        const uint32_t token = p.block_div.div(there ? item : 0u);
+        int block = (int)((there ? item : 0u) - token * p.block_div.d), which = 0;
+        if (block >= p.blocks[0]) { block -= p.blocks[0]; which = 1; if (block >= p.blocks[1]) { block -= p.blocks[1]; which = 2; } }
+        const HeadsView& h = p.part[which];
+        const int head0 = block * HB;
+        const TokenPlace at = place_token(p, (int)token, p.positions != nullptr, h.cache != nullptr);
+        const T* in = reinterpret_cast<const T*>(h.in) + at.batch * h.in_batch + at.in_row * h.in_token + head0 * h.in_head + d;
+        float x[HB][8];
+        #pragma unroll
+        for (int i = 0; i < HB; i++) {
+            if (there && mine && head0 + i < h.heads) load8(in + i * h.in_head, x[i]);
+            else {
+                #pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+            }
+        }
+        const bool normed = h.weight && mine;
+        float w[8];
+        if (normed) {
+            if (h.weight_f32) load8(reinterpret_cast<const float*>(h.weight) + d, w);
+            else load8(reinterpret_cast<const T*>(h.weight) + d, w);
+        }
+        #pragma unroll
+        for (int i = 0; i < HB; i++) {                       // the groups of a warp may be in different parts: all of them reduce
+            float sum = 0.0f;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) sum = __fmaf_rn(x[i][e], x[i][e], sum);
+            #pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            const float factor = rsqrtf(__fmaf_rn(sum, p.inv_dim, p.epsilon));
+            if (normed)
+                #pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = x[i][e] * factor * w[e];
+        }
+        if (half > 0) {
+            constexpr int N = INTERLEAVED ? 4 : 8;
+            float c[N], s[N];
+            const bool turned = h.rotate && at.table_row >= 0 && d < 2 * half;
+            if (turned) {
+                const long long row = (long long)at.table_row * half + (INTERLEAVED ? d / 2 : (second ? d - half : d));
+                #pragma unroll
+                for (int e = 0; e < N; e += 4) {
+                    const float4 cv = *reinterpret_cast<const float4*>(p.cos_table + row + e), sv = *reinterpret_cast<const float4*>(p.sin_table + row + e);
+                    c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
+                    s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < HB; i++) {
+                if constexpr (INTERLEAVED) {
+                    if (turned)
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float a = x[i][2 * e], b = x[i][2 * e + 1];
+                            x[i][2 * e] = __fmaf_rn(a, c[e], -(b * s[e]));
+                            x[i][2 * e + 1] = __fmaf_rn(a, s[e], b * c[e]);
+                        }
+                } else {
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float other = __shfl_sync(~0u, x[i][e], partner);
+                        if (turned) x[i][e] = second ? __fmaf_rn(other, s[e], x[i][e] * c[e]) : __fmaf_rn(x[i][e], c[e], -(other * s[e]));
+                    }
+                }
+            }
+        }
+        if (there && mine) {
+            T* out = h.out ? reinterpret_cast<T*>(h.out) + at.batch * h.out_batch + at.in_row * h.out_token + head0 * h.out_head + d : nullptr;
+            T* cache = h.cache && at.slot >= 0 && !at.bad_position ? reinterpret_cast<T*>(h.cache) + (at.slot * p.cache_heads + head0) * p.dim + d : nullptr;
+            #pragma unroll
+            for (int i = 0; i < HB; i++) {
+                if (head0 + i >= h.heads) break;
+                if (at.bad_position)
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+                if (out) store8(out + i * h.out_head, x[i]);
+                if (cache) store8(cache + (long long)i * p.dim, x[i]);
+            }
+        }
+    }
+}
+
+// Whether every row that the vector form reads or writes starts on a 16-byte boundary, and pairs are met lane by lane.
+static bool vector_form(const NormRotaryProblem& p) {
+    if (p.dim % 8 != 0 || p.dim > 256 || p.half % 4 != 0 || (!p.interleaved && p.half % 8 != 0)) return false;
+    uintptr_t bits = reinterpret_cast<uintptr_t>(p.cos_table) | reinterpret_cast<uintptr_t>(p.sin_table);
+    for (const HeadsView& h : p.part)
+        for (const void* a : {h.in, (const void*)h.out, (const void*)h.cache, h.weight}) bits |= reinterpret_cast<uintptr_t>(a);
+    return (bits & 15) == 0;
+}
+
+template <typename T, int LPH, int HB> static bool launch_vector(NormRotaryProblem p) {
+    DeviceState* st = acquire_device();
+    if (!st) return false;
+    int blocks = 0;
+    for (int i = 0; i < 3; i++) blocks += p.blocks[i] = (p.part[i].heads + HB - 1) / HB;
+    p.block_div.set((uint32_t)blocks);
+    const uint32_t items = (uint32_t)p.tokens * (uint32_t)blocks;
+    const int grid = grid_for(items, kNormThreads / LPH, st->sm_count, 16);
+    if (p.interleaved) norm_rotary_vector<T, LPH, HB, true><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
+    else norm_rotary_vector<T, LPH, HB, false><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
+    return TOPS_CHECK_LAUNCH("norm_rotary_vector");
+}
+
+template <typename T, int LPH> static bool launch_vector_heads(const NormRotaryProblem& p) {
+    // four heads per group share a token's table row; with few heads in all, one each spreads them over more SMs
+    const long long heads = (long long)p.tokens * (p.part[0].heads + p.part[1].heads + p.part[2].heads);
+    return heads * LPH >= (long long)kNumSMs * 2048 * 4 ? launch_vector<T, LPH, 4>(p) : launch_vector<T, LPH, 1>(p);
+}
+
+template <typename T> static bool launch_any(const NormRotaryProblem& p) {
+    if (!vector_form(p)) return launch_general<T>(p);
+    if (p.dim <= 64) return launch_vector_heads<T, 8>(p);
+    if (p.dim <= 128) return launch_vector_heads<T, 16>(p);
+    return launch_vector_heads<T, 32>(p);
+}
+
 static bool run_norm_rotary(const NormRotaryProblem& p, int dtype) {
     switch (dtype) {
-        case DTYPE_FLOAT16:  return launch_general<__half>(p);
-        case DTYPE_BFLOAT16: return launch_general<__nv_bfloat16>(p);
-        default:             return launch_general<float>(p);
+        case DTYPE_FLOAT16:  return launch_any<__half>(p);
+        case DTYPE_BFLOAT16: return launch_any<__nv_bfloat16>(p);
+        default:             return launch_any<float>(p);
     }
 }
 
@@ -171,7 +328,7 @@ TOPS_API int tops_qk_norm_rotary_forward(const QKNormRotaryCall* call) {
     const int dt = c.q->dtype;
     if (dt != DTYPE_FLOAT16 && dt != DTYPE_BFLOAT16 && dt != DTYPE_FLOAT32) return fail(TOPS_ERR_UNSUPPORTED, "float16, bfloat16 or float32");
     const size_t token_count = c.q->size / ((size_t)c.q->shape[heads_at] * (size_t)dim);
-    if (c.q->size >= 0x7FFFFFFFull * 16 || token_count >= 0x7FFFFFFFull / 64) return fail(TOPS_ERR_UNSUPPORTED, "fewer than 2^25 tokens");
+    if (token_count >= 0x7FFFFFFFull / 64) return fail(TOPS_ERR_UNSUPPORTED, "fewer than 2^25 tokens");
     // shapes of the outputs: q's with its own heads
     auto shaped = [&](const Tensor* t, int want_heads) {
         if (t->ndim != nd || t->dtype != dt) return false;
@@ -186,6 +343,7 @@ TOPS_API int tops_qk_norm_rotary_forward(const QKNormRotaryCall* call) {
         if (kv_heads < 1 || !shaped(c.k, kv_heads)) return fail(TOPS_ERR_INVALID, "k has q's shape but for the heads, and its type");
     }
     const bool keys = packed || c.k;
+    if ((unsigned long long)token_count * (unsigned long long)((long long)heads + 2ll * kv_heads) >= 0x7FFFFFFFull / 4) return fail(TOPS_ERR_UNSUPPORTED, "fewer than 2^29 heads over all tokens");
     if (c.v && (!c.k || !shaped(c.v, kv_heads))) return fail(TOPS_ERR_INVALID, "v has k's shape and type");
     if (c.k_out && (!keys || !shaped(c.k_out, kv_heads))) return fail(TOPS_ERR_INVALID, "k_out has the key heads' shape and type");
     if (keys && !c.k_out && !cached) return fail(TOPS_ERR_INVALID, "keys need k_out or a cache to go to");
