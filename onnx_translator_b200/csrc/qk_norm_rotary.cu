@@ -133,17 +133,20 @@ template <typename T> static bool launch_general(const NormRotaryProblem& p) {
 // work through HB heads of one token: all HB loads are in flight before the first use, and the token's cosines and sines are
 // read once for the HB heads.  With pairs (i, i + half) the partner elements sit in another lane of the head (a shuffle), with
 // interleaved pairs in the same lane.
-template <typename T> __device__ __forceinline__ void load8(const T* from, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(from);
-        const T* t = reinterpret_cast<const T*>(&a);
-        #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = to_float(t[i]);
-    }
+// Eight elements as they lie in memory.
+template <typename T> struct Raw8 { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Raw8<T> load_raw8(const T* from) {
+    Raw8<T> r;
+    #pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = reinterpret_cast<const uint4*>(from)[i];
+    return r;
 }
+template <typename T> __device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
+    const T* t = reinterpret_cast<const T*>(&r);
+    #pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = to_float(t[i]);
+}
+template <typename T> __device__ __forceinline__ void load8(const T* from, float (&x)[8]) { widen8(load_raw8(from), x); }
 template <typename T> __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
         reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -174,78 +177,71 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_
         if (block >= p.blocks[0]) { block -= p.blocks[0]; which = 1; if (block >= p.blocks[1]) { block -= p.blocks[1]; which = 2; } }
         const HeadsView& h = p.part[which];
         const int head0 = block * HB;
-        const TokenPlace at = place_token(p, (int)token, p.positions != nullptr, h.cache != nullptr);
-        const T* in = reinterpret_cast<const T*>(h.in) + at.batch * h.in_batch + at.in_row * h.in_token + head0 * h.in_head + d;
-        float x[HB][8];
+        const int batch = (int)p.seq_div.div(token), in_row = (int)token - batch * p.seq;
+        const T* in = reinterpret_cast<const T*>(h.in) + batch * h.in_batch + in_row * h.in_token + head0 * h.in_head + d;
+        Raw8<T> raw[HB];                                     // on their way while position, slot and table row are looked up
         #pragma unroll
-        for (int i = 0; i < HB; i++) {
-            if (there && mine && head0 + i < h.heads) load8(in + i * h.in_head, x[i]);
-            else {
-                #pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-            }
-        }
+        for (int i = 0; i < HB; i++) if (there && mine && head0 + i < h.heads) raw[i] = load_raw8(in + i * h.in_head);
         const bool normed = h.weight && mine;
         float w[8];
         if (normed) {
             if (h.weight_f32) load8(reinterpret_cast<const float*>(h.weight) + d, w);
             else load8(reinterpret_cast<const T*>(h.weight) + d, w);
         }
-        #pragma unroll
-        for (int i = 0; i < HB; i++) {                       // the groups of a warp may be in different parts: all of them reduce
-            float sum = 0.0f;
+        const TokenPlace at = place_token(p, (int)token, p.positions != nullptr, h.cache != nullptr);
+        constexpr int N = INTERLEAVED ? 4 : 8;
+        float c[N], s[N];
+        const bool turned = h.rotate && at.table_row >= 0 && d < 2 * half;
+        if (turned) {
+            const long long row = (long long)at.table_row * half + (INTERLEAVED ? d / 2 : (second ? d - half : d));
             #pragma unroll
-            for (int e = 0; e < 8; e++) sum = __fmaf_rn(x[i][e], x[i][e], sum);
+            for (int e = 0; e < N; e += 4) {
+                const float4 cv = *reinterpret_cast<const float4*>(p.cos_table + row + e), sv = *reinterpret_cast<const float4*>(p.sin_table + row + e);
+                c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
+                s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
+            }
+        }
+        T* out = h.out ? reinterpret_cast<T*>(h.out) + batch * h.out_batch + in_row * h.out_token + head0 * h.out_head + d : nullptr;
+        T* cache = h.cache && at.slot >= 0 && !at.bad_position ? reinterpret_cast<T*>(h.cache) + (at.slot * p.cache_heads + head0) * p.dim + d : nullptr;
+        #pragma unroll
+        for (int i = 0; i < HB; i++) {
+            const bool here = there && mine && head0 + i < h.heads;
+            float x[8];
+            if (here) widen8(raw[i], x);
+            else {
+                #pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = 0.0f;
+            }
+            float sum = 0.0f;                                // the groups of a warp may be in different parts: all of them reduce
+            #pragma unroll
+            for (int e = 0; e < 8; e++) sum = __fmaf_rn(x[e], x[e], sum);
             #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
             const float factor = rsqrtf(__fmaf_rn(sum, p.inv_dim, p.epsilon));
             if (normed)
                 #pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] = x[i][e] * factor * w[e];
-        }
-        if (half > 0) {
-            constexpr int N = INTERLEAVED ? 4 : 8;
-            float c[N], s[N];
-            const bool turned = h.rotate && at.table_row >= 0 && d < 2 * half;
-            if (turned) {
-                const long long row = (long long)at.table_row * half + (INTERLEAVED ? d / 2 : (second ? d - half : d));
-                #pragma unroll
-                for (int e = 0; e < N; e += 4) {
-                    const float4 cv = *reinterpret_cast<const float4*>(p.cos_table + row + e), sv = *reinterpret_cast<const float4*>(p.sin_table + row + e);
-                    c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
-                    s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
-                }
-            }
-            #pragma unroll
-            for (int i = 0; i < HB; i++) {
-                if constexpr (INTERLEAVED) {
-                    if (turned)
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float a = x[i][2 * e], b = x[i][2 * e + 1];
-                            x[i][2 * e] = __fmaf_rn(a, c[e], -(b * s[e]));
-                            x[i][2 * e + 1] = __fmaf_rn(a, s[e], b * c[e]);
-                        }
-                } else {
+                for (int e = 0; e < 8; e++) x[e] = x[e] * factor * w[e];
+            if constexpr (INTERLEAVED) {
+                if (turned)
                     #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float other = __shfl_sync(~0u, x[i][e], partner);
-                        if (turned) x[i][e] = second ? __fmaf_rn(other, s[e], x[i][e] * c[e]) : __fmaf_rn(x[i][e], c[e], -(other * s[e]));
+                    for (int e = 0; e < 4; e++) {
+                        const float a = x[2 * e], b = x[2 * e + 1];
+                        x[2 * e] = __fmaf_rn(a, c[e], -(b * s[e]));
+                        x[2 * e + 1] = __fmaf_rn(a, s[e], b * c[e]);
                     }
+            } else if (half > 0) {
+                #pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float other = __shfl_sync(~0u, x[e], partner);
+                    if (turned) x[e] = second ? __fmaf_rn(other, s[e], x[e] * c[e]) : __fmaf_rn(x[e], c[e], -(other * s[e]));
                 }
             }
-        }
-        if (there && mine) {
-            T* out = h.out ? reinterpret_cast<T*>(h.out) + at.batch * h.out_batch + at.in_row * h.out_token + head0 * h.out_head + d : nullptr;
-            T* cache = h.cache && at.slot >= 0 && !at.bad_position ? reinterpret_cast<T*>(h.cache) + (at.slot * p.cache_heads + head0) * p.dim + d : nullptr;
-            #pragma unroll
-            for (int i = 0; i < HB; i++) {
-                if (head0 + i >= h.heads) break;
+            if (here) {
                 if (at.bad_position)
                     #pragma unroll
-                    for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-                if (out) store8(out + i * h.out_head, x[i]);
-                if (cache) store8(cache + (long long)i * p.dim, x[i]);
+                    for (int e = 0; e < 8; e++) x[e] = 0.0f;
+                if (out) store8(out + i * h.out_head, x);
+                if (cache) store8(cache + (long long)i * p.dim, x);
             }
         }
     }

@@ -583,8 +583,13 @@ int* device_status_word() {
         *g_status_host = 0;
     });
     if (!g_status_host) return nullptr;
+    // the address on each device never changes: asked for once, not on every operator call
+    static std::atomic<int*> known[kMaxDevices];
+    const int device = current_device_index();
+    if (device >= 0 && device < kMaxDevices) if (int* p = known[device].load(std::memory_order_relaxed)) return p;
     int* dev = nullptr;
     if (cudaHostGetDevicePointer((void**)&dev, g_status_host, 0) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+    if (device >= 0 && device < kMaxDevices) known[device].store(dev, std::memory_order_relaxed);
     return dev;
 }
 
