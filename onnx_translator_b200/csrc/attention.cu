@@ -48,8 +48,28 @@ static bool whole_pieces(const AttentionProblem& p) {
     return p.dtype != DTYPE_FLOAT32 && p.dim % 8 == 0 && (bits & 15) == 0;
 }
 
+int cache_box_rows(const AttentionProblem& p) {
+    if (!p.page_table) return 128;
+    if (p.pages == 0) return 0;                              // no cache to describe
+    if (p.page_size % 128 == 0) return 128;
+    return p.page_size % 8 == 0 && 128 % p.page_size == 0 ? p.page_size : 0;
+}
+
+bool make_cache_map(CUtensorMap* map, const AttentionProblem& p, const void* base, int box_rows) {
+    const bool paged = p.page_table != nullptr;
+    const uint64_t rows = paged ? (uint64_t)p.pages * p.page_size : (uint64_t)p.keys;
+    const uint64_t dims[4] = {(uint64_t)p.dim, (uint64_t)p.kv_heads, rows, paged ? 1u : (uint64_t)p.batch};
+    const uint64_t strides[3] = {(uint64_t)p.kv_head * 2, (uint64_t)p.kv_token * 2, paged ? rows * (uint64_t)p.kv_token * 2 : (uint64_t)p.kv_batch * 2};
+    const uint32_t box[4] = {64, 1, (uint32_t)box_rows, 1};
+    return make_tensor_map(map, base, 2, false, p.dtype == DTYPE_FLOAT16, 4, dims, strides, box, nullptr);
+}
+
 static bool run_attention(const AttentionProblem& p) {
-    if (whole_pieces(p)) return attention_rows(p);
+    if (whole_pieces(p)) {
+        const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
+        if (cache_box_rows(p) > 0 && rows <= 64) return attention_step(p);
+        return attention_rows(p);
+    }
     return attention_fma(p);
 }
 

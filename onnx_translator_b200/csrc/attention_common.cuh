@@ -12,6 +12,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "umma.cuh"
 
 namespace tops {
 
@@ -286,6 +287,12 @@ int attention_splits(const AttentionProblem& p, long long tiles, int blocks_want
 long long attention_tiles(const AttentionProblem& p, int rows_per_tile);
 bool launch_attention(const void* kernel, const AttentionProblem& p, int rows_per_tile, int threads, size_t smem, int splits, void** args, const char* name);
 
+// Tensor map over k or v: (dim, head, row, batch) in boxes of 64 x 1 x box_rows x 1, 128-byte swizzle; dims past the head are zeros.
+bool make_cache_map(CUtensorMap* map, const AttentionProblem& p, const void* base, int box_rows);
+// Rows of a box that stay inside a page (dense: 128): a divisor of 128 that is a multiple of the 8-row swizzle group; 0 if there is none.
+int cache_box_rows(const AttentionProblem& p);
+
+bool attention_step(const AttentionProblem& p);      // 16-bit types, cache_box_rows > 0: up to 64 rows per block, tcgen05
 bool attention_fma(const AttentionProblem& p);       // any type, any dim up to 256
 bool attention_rows(const AttentionProblem& p);      // 16-bit types, dim % 8 == 0: 16 rows per block, mma.sync
 

@@ -156,6 +156,25 @@ template <int W> __device__ __forceinline__ void tmem_load_chunk(uint32_t taddr,
     if constexpr (W == 32) tmem_load_32x32(taddr, r);
     else tmem_load_32x16(taddr, r);
 }
+// The stores that go with them.
+__device__ __forceinline__ void tmem_store_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_store_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---- descriptors ----------------------------------------------------------------------------------------------
@@ -166,6 +185,15 @@ __device__ __forceinline__ uint64_t smem_desc_k_major_sw128(const void* tile) {
     const uint64_t addr = (uint64_t)(smem_u32(tile) & 0x3FFFFu) >> 4;
     return addr | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+// The same bytes seen with the 128-byte rows as the K dimension (an MN-major operand): a row holds 64 elements of M (or N),
+// eight rows make a swizzle group 1024 bytes from the next (stride byte offset), and the next 64 elements of M lie
+// `block_bytes` further (leading byte offset; 0 repeats the first 64).
+__device__ __forceinline__ uint64_t smem_desc_mn_major_sw128(const void* tile, uint32_t block_bytes) {
+    const uint64_t addr = (uint64_t)(smem_u32(tile) & 0x3FFFFu) >> 4;
+    return addr | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Bits of the instruction descriptor that declare an operand MN-major.
+constexpr uint32_t kInstrAMnMajor = 1u << 15, kInstrBMnMajor = 1u << 16;
 // Instruction descriptor: fp32 accumulate, both operands K-major, dense.
 // format codes: kind f16 -> 0 fp16, 1 bf16; kind f8f6f4 -> 0 e4m3, 1 e5m2.
 __host__ __device__ constexpr uint32_t instr_desc(uint32_t a_format, uint32_t b_format, uint32_t m, uint32_t n) {
