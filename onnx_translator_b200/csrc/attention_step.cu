@@ -12,6 +12,9 @@
 // 2^8, the sums are float32, and the quotient o / l does not depend on m.  When the check fails, about ln(tiles) times per row, the block
 // takes the true maximum and rescales o and l.  Sums of weights stay per thread (per key) until the end.
 //
+// Rows are worked on four at a time: the columns between t.rows and the next multiple of four hold scores of zero queries and are dropped
+// at the end (a branch per row cost more than the arithmetic of three idle ones).
+//
 // Warps 0-3 softmax, warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs.  Blocks of a cluster share a
 // sequence's keys and join at the end; tensor memory is given back before that, so a block that waits for its peers holds none.
 #include "attention_common.cuh"
@@ -33,6 +36,7 @@ template <int DB, int N, int SLOTS> struct StepLayout {
     static constexpr int kSmem = SLOTS * kSlotBytes + kQBytes + 2 * kPBytes + 1024;   // and room to align
     static constexpr int kOAccs = DB > 2 ? 2 : 1;             // accumulators of 128 dimensions
     static constexpr uint32_t kColumns = (2 + kOAccs) * N <= 64 ? 64 : (2 + kOAccs) * N <= 128 ? 128 : 256;
+    static_assert(SLOTS <= 8, "a slot's release is read from barriers of the last four tiles");
     static_assert(N * kPitch * 4 <= SLOTS * kSlotBytes, "the partial result reuses the ring");
 };
 
@@ -88,7 +92,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                       const __grid_constant__ AttentionProblem p, const int tiles, const int box_rows) {
     using L = StepLayout<DB, N, SLOTS>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[SLOTS], empty[SLOTS], s_full[2], p_ready[2], pv_done[2], drained;
+    __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word, drain_word;
     __shared__ float warp_top[4][N], fade[N], warp_sum[4][N];
@@ -112,35 +116,46 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
 
     // Copies (warp 4): load number g is the keys (g even) or values (g odd) of tile g / 2 of this block, into ring slot g % SLOTS.  The first SLOTS
     // of them need no slot to be given back and are started before the block has even met.
-    int g = 0, box_row = -1, next_box_row = -1;
+    int g = 0, box_row = -1, next_page = 0;
     uint32_t load_slot = 0, load_phase = 0;
-    auto page_row = [&](int tile) {                            // cache row of this lane's box of a tile; -1: nothing to copy
+    // A tile's pages are fetched a tile ahead and looked at only when the tile's turn comes, so that the copies never wait for the table.
+    auto box_needed = [&](int tile, int j) { return tile < hi && lane * box_rows < kStepKeys && j < t.key_end; };
+    auto fetch_page = [&](int tile) {
         const int j = tile * kStepKeys + lane * box_rows;
-        if (tile >= hi || lane * box_rows >= kStepKeys || j >= t.key_end) return -1;
-        if (!p.page_table) return j;
-        if (j + box_rows <= t.key_begin) return p.pages * p.page_size;              // in front of the window: the page may be gone, zeros will do
-        const int row = key_row(p, t.seq, j);
-        return row >= 0 ? row : p.pages * p.page_size;                                // outside the map: zeros
+        const bool needed = p.page_table && box_needed(tile, j) && j + box_rows > t.key_begin;     // pages in front of a window may be gone
+        return needed ? p.page_table[(long long)t.seq * p.table_width + (int)p.page_div.div((uint32_t)j)] : 0;
     };
-    auto load = [&](bool wait) {                               // the whole warp; false when the block gives up
-        uint32_t ok = 1;
-        const uint32_t boxes = (uint32_t)__popc(__ballot_sync(~0u, box_row >= 0));
-        if (lane == 0) {
-            if (wait) ok = umma::mbar_wait(&empty[load_slot], load_phase ^ 1u, abort_flag);
-            if (ok) umma::mbar_expect_tx(&full[load_slot], boxes * (uint32_t)box_rows * 128u * DB);
+    auto page_row = [&](int tile, int page) {                  // cache row of this lane's box of a tile; -1: nothing to copy
+        const int j = tile * kStepKeys + lane * box_rows;
+        if (!box_needed(tile, j)) return -1;
+        if (!p.page_table) return j;
+        const int outside = p.pages * p.page_size;             // a row outside the map reads as zeros
+        if (j + box_rows <= t.key_begin) return outside;
+        if ((unsigned)page >= (unsigned)p.pages) { report_bad_index(p); return outside; }
+        return page * p.page_size + (j - (int)p.page_div.div((uint32_t)j) * p.page_size);
+    };
+    auto load = [&] {                                          // the whole warp; false when the block gives up
+        if (g >= SLOTS) {                                      // the slot's last contents: keys are read out with their scores, values with their product
+            const int old = g - SLOTS, i = old >> 1;
+            if (!__all_sync(~0u, umma::mbar_wait((old & 1) ? &pv_done[i & 3] : &s_full[i & 3], (uint32_t)(i >> 2) & 1u, abort_flag))) return false;
         }
-        ok = __shfl_sync(~0u, ok, 0);
-        if (!ok) return false;
-        if (box_row >= 0) {
-            #pragma unroll
-            for (int b = 0; b < DB; b++)
-                umma::tma_load_4d(ring + load_slot * L::kSlotBytes + b * (kStepKeys * 128) + lane * box_rows * 128, (g & 1) ? &v_map : &k_map, &full[load_slot],
-                                  b * 64, kv_head, box_row, p.page_table ? 0 : t.seq);
-        }
+        const int boxes = __popc(__ballot_sync(~0u, box_row >= 0));
+        uint8_t* to = ring + load_slot * L::kSlotBytes;
+        const CUtensorMap* map = (g & 1) ? &v_map : &k_map;
+        const int batch = p.page_table ? 0 : t.seq;
+        if (umma::elect_one()) umma::mbar_expect_tx(&full[load_slot], (uint32_t)(boxes * box_rows) * 128u * DB);
         __syncwarp();
-        if (g & 1) {                                           // the next tile's pages were looked up a tile ago
-            box_row = next_box_row;
-            next_box_row = page_row(lo + (g >> 1) + 2);
+        for (int x = 0; x < boxes; x++) {
+            const int row = __shfl_sync(~0u, box_row, x);
+            if (umma::elect_one()) {
+                #pragma unroll
+                for (int b = 0; b < DB; b++) umma::tma_load_4d(to + b * (kStepKeys * 128) + x * box_rows * 128, map, &full[load_slot], b * 64, kv_head, row, batch);
+            }
+            __syncwarp();
+        }
+        if (g & 1) {
+            box_row = page_row(lo + (g >> 1) + 1, next_page);
+            next_page = fetch_page(lo + (g >> 1) + 2);
         }
         g++;
         if (++load_slot == SLOTS) { load_slot = 0; load_phase ^= 1u; }
@@ -148,16 +163,18 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     };
     if (warp == 4) {
         if (lane == 0) {
-            for (int s = 0; s < SLOTS; s++) { umma::mbar_init(&full[s], 1); umma::mbar_init(&empty[s], 1); }
-            for (int b = 0; b < 2; b++) { umma::mbar_init(&s_full[b], 1); umma::mbar_init(&p_ready[b], 128); umma::mbar_init(&pv_done[b], 1); }
+            for (int s = 0; s < SLOTS; s++) umma::mbar_init(&full[s], 1);
+            for (int b = 0; b < 4; b++) { umma::mbar_init(&s_full[b], 1); umma::mbar_init(&pv_done[b], 1); }
+            for (int b = 0; b < 2; b++) umma::mbar_init(&p_ready[b], 128);
             umma::mbar_init(&drained, 1);
             abort_word = drain_word = 0;
             umma::mbar_fence_init();
         }
         __syncwarp();
-        box_row = page_row(lo);
-        next_box_row = page_row(lo + 1);
-        while (g < 2 * n && g < SLOTS) load(false);
+        box_row = fetch_page(lo);
+        next_page = fetch_page(lo + 1);
+        box_row = page_row(lo, box_row);
+        while (g < 2 * n && g < SLOTS) load();
     }
 
     // queries and zeroed weights into shared memory, the N rows 128 bytes each, 16-byte pieces XORed with the row as the swizzle wants
@@ -167,6 +184,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         if (r < t.rows && c * 8 < p.dim) x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + row_offset(p, t, kv_head, t.row0 + r) + c * 8);
         *reinterpret_cast<uint4*>(q_tile + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
     }
+    if (threadIdx.x < N) fade[threadIdx.x] = 1.0f;            // of the columns that no row uses
     for (int i = threadIdx.x; i < 2 * L::kPBytes / 16; i += kStepThreads) reinterpret_cast<uint4*>(p_tile)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x < N)
         high[threadIdx.x] = p.page_table ? t.first_position + (int)p.group_div.div((uint32_t)(t.row0 + min((int)threadIdx.x, t.rows - 1))) + 1 : t.key_end;
@@ -177,7 +195,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     const uint32_t tmem = tmem_slot, tmem_o = tmem + 2 * N;
 
     if (warp == 4) {
-        while (g < 2 * n && load(true)) {}
+        while (g < 2 * n && load()) {}
         if (lane == 0) {                                       // no copy of this block is in flight when it leaves
             for (int k = min(g, SLOTS); k > 0; k--) {
                 if (load_slot == 0) { load_slot = SLOTS; load_phase ^= 1u; }
@@ -186,50 +204,52 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             }
         }
     } else if (warp == 5) {
-        if (lane == 0) {
-            // ---- products ------------------------------------------------------------------------------------------------
-            const uint32_t fmt = sizeof(T) == 2 && (std::is_same<T, __nv_bfloat16>::value) ? 1u : 0u;
-            const uint32_t idesc_s = umma::instr_desc(fmt, fmt, 128, N), idesc_o = umma::instr_desc(fmt, fmt, 128, N) | umma::kInstrAMnMajor;
-            uint32_t slot = 0, phase = 0;
-            bool ok = true;
-            auto scores = [&](int i) {                         // S^T of tile i
-                if (!umma::mbar_wait(&full[slot], phase, abort_flag)) return false;
-                umma::fence_after_sync();
+        // ---- products: the whole warp waits, one elected lane issues --------------------------------------------------------
+        constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t idesc_s = umma::instr_desc(fmt, fmt, 128, N), idesc_o = idesc_s | umma::kInstrAMnMajor;
+        uint32_t slot = 0, phase = 0;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, umma::mbar_wait(bar, parity, abort_flag)); };
+        auto scores = [&](int i) {                             // S^T of tile i
+            if (!wait(&full[slot], phase)) return false;
+            umma::fence_after_sync();
+            const uint64_t da = umma::smem_desc_k_major_sw128(ring + slot * L::kSlotBytes), db = umma::smem_desc_k_major_sw128(q_tile);
+            if (umma::elect_one()) {
                 #pragma unroll
-                for (int b = 0; b < DB; b++) {
-                    const uint64_t da = umma::smem_desc_k_major_sw128(ring + slot * L::kSlotBytes + b * (kStepKeys * 128));
-                    const uint64_t db = umma::smem_desc_k_major_sw128(q_tile + b * (N * 128));
+                for (int b = 0; b < DB; b++)
                     #pragma unroll
-                    for (int k = 0; k < 4; k++) umma::mma_ss<false>(tmem + (i & 1) * N, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_s, (uint32_t)(b | k));
-                }
-                umma::mma_commit(&empty[slot]);
-                umma::mma_commit(&s_full[i & 1]);
-                return true;
-            };
-            auto step = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1u; } };
-            if (n > 0) ok = scores(0);
-            for (int i = 0; i < n && ok; i++) {
-                step();                                        // this tile's values
-                const uint32_t v_slot = slot, v_phase = phase;
-                step();                                        // the next tile's keys
-                if (i + 1 < n && !scores(i + 1)) { ok = false; break; }
-                if (!umma::mbar_wait(&p_ready[i & 1], (uint32_t)(i >> 1) & 1u, abort_flag)) { ok = false; break; }
-                if (!umma::mbar_wait(&full[v_slot], v_phase, abort_flag)) { ok = false; break; }
-                umma::fence_after_sync();
-                #pragma unroll
-                for (int a = 0; a < L::kOAccs; a++) {
-                    const uint8_t* v_tile = ring + v_slot * L::kSlotBytes + a * 2 * (kStepKeys * 128);
-                    const uint64_t da = umma::smem_desc_mn_major_sw128(v_tile, DB == 1 ? 0u : (uint32_t)(kStepKeys * 128));
-                    #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const uint64_t db = umma::smem_desc_k_major_sw128(p_tile + (i & 1) * L::kPBytes + (k >> 2) * (N * 128)) + (uint64_t)(2 * (k & 3));
-                        umma::mma_ss<false>(tmem_o + a * N, da + (uint64_t)(k * (2048 >> 4)), db, idesc_o, (uint32_t)(i | k));
-                    }
-                }
-                umma::mma_commit(&empty[v_slot]);
-                umma::mma_commit(&pv_done[i & 1]);
+                    for (int k = 0; k < 4; k++)
+                        umma::mma_ss<false>(tmem + (i & 1) * N, da + (uint64_t)(b * (kStepKeys * 128 >> 4) + 2 * k), db + (uint64_t)(b * (N * 128 >> 4) + 2 * k), idesc_s, (uint32_t)(b | k));
+                umma::mma_commit(&s_full[i & 3]);
             }
-            if (!ok) { umma::mma_commit(&drained); umma::mbar_wait(&drained, 0, &drain_word); }
+            __syncwarp();
+            return true;
+        };
+        auto step = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1u; } };
+        bool ok = n > 0 ? scores(0) : true;
+        for (int i = 0; i < n && ok; i++) {
+            step();                                            // this tile's values
+            const uint32_t v_slot = slot, v_phase = phase;
+            step();                                            // the next tile's keys
+            ok = (i + 1 == n || scores(i + 1)) && wait(&p_ready[i & 1], (uint32_t)(i >> 1) & 1u) && wait(&full[v_slot], v_phase);
+            if (!ok) break;
+            umma::fence_after_sync();
+            const uint64_t da = umma::smem_desc_mn_major_sw128(ring + v_slot * L::kSlotBytes, DB == 1 ? 0u : (uint32_t)(kStepKeys * 128));
+            const uint64_t db = umma::smem_desc_k_major_sw128(p_tile + (i & 1) * L::kPBytes);
+            if (umma::elect_one()) {
+                #pragma unroll
+                for (int a = 0; a < L::kOAccs; a++)
+                    #pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        umma::mma_ss<false>(tmem_o + a * N, da + (uint64_t)(a * 2 * (kStepKeys * 128 >> 4) + k * (2048 >> 4)),
+                                            db + (uint64_t)((k >> 2) * (N * 128 >> 4) + 2 * (k & 3)), idesc_o, (uint32_t)(i | k));
+                umma::mma_commit(&pv_done[i & 3]);
+            }
+            __syncwarp();
+        }
+        if (!ok) {
+            if (umma::elect_one()) umma::mma_commit(&drained);
+            __syncwarp();
+            umma::mbar_wait(&drained, 0, &drain_word);
         }
     } else {
         // ---- softmax: a thread per key -------------------------------------------------------------------------------------
@@ -256,62 +276,70 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 dead = j >= t.key_end;
                 if (masked && !dead) { bias = key_bias(p, t.seq, j); dead = bias == -INFINITY; }
             }
-            if (!umma::mbar_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, abort_flag)) ok = false;
+            if (!umma::mbar_wait(&s_full[i & 3], (uint32_t)(i >> 2) & 1u, abort_flag)) ok = false;
             umma::fence_after_sync();
             float z[N];
             tmem_load_columns<N>(tmem + lanes + (i & 1) * N, z);
             float over = -INFINITY;
             if (!edge) {
                 #pragma unroll
-                for (int r = 0; r < N; r++) if (r < t.rows) { z[r] *= p.scale_log2; over = fmaxf(over, z[r] - m[r]); }
+                for (int c = 0; c < N; c += 4)
+                    if (c < t.rows)
+                        #pragma unroll
+                        for (int r = c; r < c + 4; r++) { z[r] *= p.scale_log2; over = fmaxf(over, z[r] - m[r]); }
             } else {
                 #pragma unroll
-                for (int r = 0; r < N; r++) if (r < t.rows) {
-                    const bool seen = !dead && j < high[r] && (p.window == 0 || j >= high[r] - p.window);
-                    z[r] = seen ? __fmaf_rn(z[r], p.scale_log2, bias) : -INFINITY;
-                    over = fmaxf(over, z[r] - m[r]);
-                }
+                for (int c = 0; c < N; c += 4)
+                    if (c < t.rows)
+                        #pragma unroll
+                        for (int r = c; r < c + 4; r++) {
+                            const bool seen = !dead && j < high[r] && (p.window == 0 || j >= high[r] - p.window);
+                            z[r] = seen ? __fmaf_rn(z[r], p.scale_log2, bias) : -INFINITY;
+                            over = fmaxf(over, z[r] - m[r]);
+                        }
             }
             if (any_of_softmax(over > kMaximumSlack)) {
                 #pragma unroll
-                for (int r = 0; r < N; r++) {
-                    if (r < t.rows) {
-                        float top = z[r];
+                for (int c = 0; c < N; c += 4)
+                    if (c < t.rows)
                         #pragma unroll
-                        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                        if (lane == 0) warp_top[warp][r] = top;
-                    }
-                }
+                        for (int r = c; r < c + 4; r++) {
+                            float top = z[r];
+                            #pragma unroll
+                            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                            if (lane == 0) warp_top[warp][r] = top;
+                        }
                 softmax_sync();
                 #pragma unroll
-                for (int r = 0; r < N; r++) {
-                    float f = 1.0f;
-                    if (r < t.rows) {
-                        const float top = fmaxf(m[r], fmaxf(fmaxf(warp_top[0][r], warp_top[1][r]), fmaxf(warp_top[2][r], warp_top[3][r])));
-                        f = exp2_approx(m[r] - top);
-                        l[r] *= f;
-                        m[r] = top;
-                    }
-                    if (key == r) fade[r] = f;
-                }
+                for (int c = 0; c < N; c += 4)
+                    if (c < t.rows)
+                        #pragma unroll
+                        for (int r = c; r < c + 4; r++) {
+                            const float top = fmaxf(m[r], fmaxf(fmaxf(warp_top[0][r], warp_top[1][r]), fmaxf(warp_top[2][r], warp_top[3][r])));
+                            const float f = exp2_approx(m[r] - top);
+                            l[r] *= f;
+                            m[r] = top;
+                            if (key == r) fade[r] = f;
+                        }
                 softmax_sync();
                 if (i > 0) {
-                    if (!umma::mbar_wait(&pv_done[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u, abort_flag)) ok = false;
+                    if (!umma::mbar_wait(&pv_done[(i - 1) & 3], (uint32_t)((i - 1) >> 2) & 1u, abort_flag)) ok = false;
                     umma::fence_after_sync();
                     #pragma unroll
                     for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<N>(tmem_o + lanes + a * N, fade);
                 }
             }
-            if (i > 1 && !umma::mbar_wait(&pv_done[i & 1], (uint32_t)((i >> 1) - 1) & 1u, abort_flag)) ok = false;    // the weights of tile i - 2 are read
+            if (i > 1 && !umma::mbar_wait(&pv_done[(i - 2) & 3], (uint32_t)((i - 2) >> 2) & 1u, abort_flag)) ok = false;    // the weights of tile i - 2 are read
             uint8_t* to = p_tile + (i & 1) * L::kPBytes + (key >> 6) * (N * 128) + (key & 7) * 2;
             #pragma unroll
-            for (int r = 0; r < N; r++) {
-                if (r < t.rows) {
-                    const float w = exp2_approx(z[r] - m[r]);
-                    l[r] += w;
-                    *reinterpret_cast<T*>(to + r * 128 + ((((key & 63) >> 3) ^ (r & 7)) << 4)) = from_float<T>(w);
-                }
-            }
+            for (int c = 0; c < N; c += 4)
+                if (c < t.rows)
+                    #pragma unroll
+                    for (int r = c; r < c + 4; r++) {
+                        const float w = exp2_approx(z[r] - m[r]);
+                        l[r] += w;
+                        *reinterpret_cast<T*>(to + r * 128 + ((((key & 63) >> 3) ^ (r & 7)) << 4)) = from_float<T>(w);
+                    }
             if (dead) {                                        // a weight of zero times a NaN would still be one
                 if (!umma::mbar_wait(&full[slot], phase, abort_flag)) ok = false;
                 uint8_t* row = ring + slot * L::kSlotBytes + key * 128;
@@ -327,7 +355,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             if (!ok) break;
         }
         if (n > 0) {
-            if (ok) ok = umma::mbar_wait(&pv_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag);
+            if (ok) ok = umma::mbar_wait(&pv_done[(n - 1) & 3], (uint32_t)((n - 1) >> 2) & 1u, abort_flag);
             umma::fence_after_sync();
         }
         // o[r][d] into the ring (everything in it has been read), the sums of weights across the keys
