@@ -3,20 +3,24 @@
 //
 // The scores are computed transposed, so that the many keys fill the 128 rows of the instruction and the few queries its N columns:
 //   S^T[128 keys x N] = K[128 x dim] Q^T,      O^T[dim x N] += V^T[dim x 128] P^T
-// K is the A operand as it lies in memory; V, [keys][dim], is A seen MN-major; Q and P are K-major B operands of N rows.  Both
-// products take N = 16 columns for up to 16 rows: an eighth of the tensor time of a tile whose rows are the queries, and a thread
-// of the softmax owns one key -- its mask, its visibility -- with the N scores of that key in registers.
+// K is the A operand as it lies in memory; V, [keys][dim], is A seen MN-major; Q and P are K-major B operands of N rows.  A thread of the softmax owns
+// one key -- its mask, its visibility -- with the N scores of that key in registers.
 //
 // The maximum of a row would have to be taken across the threads.  Instead all rows keep a running reference m, and a tile only checks
 // (one predicate, or-reduced by the barrier it needs anyway) that no score exceeds m by more than 8 in log2: the weights stay below
 // 2^8, the sums are float32, and the quotient o / l does not depend on m.  When the check fails, about ln(tiles) times per row, the block
 // takes the true maximum and rescales o and l.  Sums of weights stay per thread (per key) until the end.
-//
 // Rows are worked on four at a time: the columns between t.rows and the next multiple of four hold scores of zero queries and are dropped
 // at the end (a branch per row cost more than the arithmetic of three idle ones).
 //
-// Warps 0-3 softmax, warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs.  Blocks of a cluster share a
-// sequence's keys and join at the end; tensor memory is given back before that, so a block that waits for its peers holds none.
+// Work is split evenly whatever the lengths: all 128-key tiles of all (sequence, key head) items stand in one row, and block c takes the c-th share of
+// it, possibly the end of one item, some whole items and the beginning of another.  The pipeline runs on across items.  An item that lies inside one share
+// is stored at once; of an item that spans several, each block leaves (m, l, o) in scratch memory, at most two per block, and a
+// second small kernel joins them in the order of the keys.  (Clusters that join through distributed shared memory were measured first: the GPU
+// holds only 15 clusters of eight such blocks at a time, 120 of 148 SMs, and 16 items then took two rounds: 235 us where this takes REPLACE_LONG.)
+//
+// Warps 0-3 softmax, warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs, warp 6 finds the next item and brings
+// its queries.
 #include "attention_common.cuh"
 
 #include <type_traits>
@@ -25,19 +29,121 @@ namespace tops {
 
 void count_tensor_core_launch();
 
-constexpr int kStepThreads = 192;
+constexpr int kStepThreads = 224;
 constexpr int kStepKeys = 128;
 
 template <int DB, int N, int SLOTS> struct StepLayout {
     static constexpr int kSlotBytes = kStepKeys * 128 * DB;
-    static constexpr int kQBytes = N * 128 * DB;
+    static constexpr int kQBytes = N * 128 * DB;              // one of the two buffers
     static constexpr int kPBytes = N * 128 * 2;               // one of the two buffers
-    static constexpr int kPitch = DB * 64 + 4;
-    static constexpr int kSmem = SLOTS * kSlotBytes + kQBytes + 2 * kPBytes + 1024;   // and room to align
+    static constexpr int kDims = DB * 64;
+    static constexpr int kSmem = SLOTS * kSlotBytes + 2 * kQBytes + 2 * kPBytes + 1024;   // and room to align
     static constexpr int kOAccs = DB > 2 ? 2 : 1;             // accumulators of 128 dimensions
     static constexpr uint32_t kColumns = (2 + kOAccs) * N <= 64 ? 64 : (2 + kOAccs) * N <= 128 ? 128 : 256;
     static_assert(SLOTS <= 8, "a slot's release is read from barriers of the last four tiles");
-    static_assert(N * kPitch * 4 <= SLOTS * kSlotBytes, "the partial result reuses the ring");
+};
+
+// ---- the row of all tiles ------------------------------------------------------------------------------------------------
+// Sequence b has tiles_of_rows row tiles of N rows; each of them, for each key head, counts `units` 128-key tiles (at least one, so that
+// rows without a key are visited as well).
+struct SequenceWork { int start, tokens, length, units, row_tiles; };
+
+template <int N> __device__ __forceinline__ SequenceWork sequence_work(const AttentionProblem& p, int b) {
+    SequenceWork w = {0, 0, 0, 0, 0};
+    if (b >= p.batch) return w;
+    int first_key = 0;
+    if (p.page_table) {
+        const int s = p.query_start[b], e = p.query_start[b + 1], length = p.kv_length[b];
+        w.start = min(max(s, 0), p.queries);
+        const int end = min(max(e, w.start), p.queries);
+        w.tokens = end - w.start;
+        w.length = min(max(length, 0), p.keys);
+        if (w.start != s || end != e || w.length != length) report_bad_index(p);
+        if (p.window > 0) first_key = max(0, w.length - w.tokens - p.window + 1);
+    } else {
+        w.tokens = p.queries;
+        w.length = p.kv_length ? min(max(p.kv_length[b], 0), p.keys) : p.keys;
+    }
+    w.row_tiles = (w.tokens * p.group + N - 1) / N;
+    w.units = max(1, (w.length + kStepKeys - 1) / kStepKeys - first_key / kStepKeys);
+    return w;
+}
+
+// Where a unit of that row lies: row tile, key head and unit inside them.
+struct UnitPlace { SequenceWork w; int seq, row_tile, kv_head, unit; };
+
+// All units; called by whole warps.
+template <int N> __device__ __forceinline__ int total_units(const AttentionProblem& p) {
+    int sum = 0;
+    for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
+        const SequenceWork w = sequence_work<N>(p, b);
+        sum += w.row_tiles * w.units;
+    }
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    return sum * p.kv_heads;
+}
+
+template <int N> __device__ __forceinline__ UnitPlace place_unit(const AttentionProblem& p, int x) {
+    const int lane = threadIdx.x & 31;
+    UnitPlace at = {};
+    int before = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+        const SequenceWork w = sequence_work<N>(p, base + lane);
+        const int mine = w.row_tiles * w.units * p.kv_heads;
+        int sum = mine;
+        #pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(~0u, sum, d); if (lane >= d) sum += o; }
+        const unsigned past = __ballot_sync(~0u, x < before + sum);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            at.seq = base + l;
+            at.w.start = __shfl_sync(~0u, w.start, l);
+            at.w.tokens = __shfl_sync(~0u, w.tokens, l);
+            at.w.length = __shfl_sync(~0u, w.length, l);
+            at.w.units = __shfl_sync(~0u, w.units, l);
+            at.w.row_tiles = __shfl_sync(~0u, w.row_tiles, l);
+            const int inside = x - before - __shfl_sync(~0u, sum - mine, l);
+            const int item = inside / at.w.units;
+            at.unit = inside - item * at.w.units;
+            at.row_tile = item / p.kv_heads;
+            at.kv_head = item - at.row_tile * p.kv_heads;
+            break;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+    }
+    return at;
+}
+
+template <int N> __device__ __forceinline__ RowTile row_tile_of(const AttentionProblem& p, const UnitPlace& at) {
+    RowTile t;
+    t.seq = at.seq;
+    t.row0 = at.row_tile * N;
+    t.rows = min(N, at.w.tokens * p.group - t.row0);
+    t.token0 = at.w.start;
+    t.length = t.key_end = at.w.length;
+    t.key_begin = 0;
+    if (p.page_table) {
+        t.first_position = at.w.length - at.w.tokens;
+        const int first = t.first_position + (int)p.group_div.div((uint32_t)t.row0);
+        const int last = t.first_position + (int)p.group_div.div((uint32_t)(t.row0 + t.rows - 1));
+        t.key_end = max(0, min(t.length, last + 1));
+        if (p.window > 0) t.key_begin = min(max(0, first - p.window + 1), t.key_end);
+    }
+    return t;
+}
+
+// First 128-key tile of an item's units.
+__device__ __forceinline__ int first_tile_of(const AttentionProblem& p, const UnitPlace& at) {
+    return p.window > 0 && p.page_table ? max(0, at.w.length - at.w.tokens - p.window + 1) / kStepKeys : 0;
+}
+
+struct Segment {
+    RowTile t;
+    int kv_head;
+    int lo, n;                   // 128-key tiles lo .. lo + n - 1; n < 0: no more segments
+    int part;                    // scratch slot of the partial result, -1: the item is whole
+    int pages[16];               // pages of tile lo
 };
 
 // True for all 128 softmax threads if it is for one.
@@ -89,148 +195,215 @@ constexpr float kMaximumSlack = 8.0f;
 template <typename T, int DB, int N, int SLOTS>
 __global__ void __launch_bounds__(kStepThreads)
 attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                      const __grid_constant__ AttentionProblem p, const int tiles, const int box_rows) {
+                      const __grid_constant__ AttentionProblem p, const int box_rows, float* __restrict__ part_o, float2* __restrict__ part_stats) {
     using L = StepLayout<DB, N, SLOTS>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], drained;
+    __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], seg_full[2], seg_empty[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word, drain_word;
-    __shared__ float warp_top[4][N], fade[N], warp_sum[4][N];
+    __shared__ __align__(16) unsigned char segment_memory[2 * sizeof(Segment)];
+    Segment* segments = reinterpret_cast<Segment*>(segment_memory);
+    __shared__ __align__(16) float warp_top[4][N], fade[N], top_of[N], sums[N];
     __shared__ int high[N];
-    __shared__ float2 stats[N];
     uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t* q_tile = ring + SLOTS * L::kSlotBytes;
-    uint8_t* p_tile = q_tile + L::kQBytes;
-
-    const int splits = (int)cluster_size(), rank = (int)cluster_rank();
-    const int kv_head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    RowTile t;
-    if (!locate_tile(p, tiles - 1 - (int)(blockIdx.x / (unsigned)splits), N, t)) return;    // the whole cluster leaves
-
-    if (warp == 5) umma::tmem_alloc(&tmem_slot, L::kColumns);
+    uint8_t* q_tiles = ring + SLOTS * L::kSlotBytes;
+    uint8_t* p_tile = q_tiles + 2 * L::kQBytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &abort_word;
 
-    const int first = t.key_begin / kStepKeys, count = (t.key_end + kStepKeys - 1) / kStepKeys - first;
-    const int share = (count + splits - 1) / splits;
-    const int lo = first + min(rank * share, count), hi = first + min((rank + 1) * share, count), n = hi - lo;
-
-    // Copies (warp 4): load number g is the keys (g even) or values (g odd) of tile g / 2 of this block, into ring slot g % SLOTS.  The first SLOTS
-    // of them need no slot to be given back and are started before the block has even met.
-    int g = 0, box_row = -1, next_page = 0;
-    uint32_t load_slot = 0, load_phase = 0;
-    // A tile's pages are fetched a tile ahead and looked at only when the tile's turn comes, so that the copies never wait for the table.
-    auto box_needed = [&](int tile, int j) { return tile < hi && lane * box_rows < kStepKeys && j < t.key_end; };
-    auto fetch_page = [&](int tile) {
-        const int j = tile * kStepKeys + lane * box_rows;
-        const bool needed = p.page_table && box_needed(tile, j) && j + box_rows > t.key_begin;     // pages in front of a window may be gone
-        return needed ? p.page_table[(long long)t.seq * p.table_width + (int)p.page_div.div((uint32_t)j)] : 0;
-    };
-    auto page_row = [&](int tile, int page) {                  // cache row of this lane's box of a tile; -1: nothing to copy
-        const int j = tile * kStepKeys + lane * box_rows;
-        if (!box_needed(tile, j)) return -1;
-        if (!p.page_table) return j;
-        const int outside = p.pages * p.page_size;             // a row outside the map reads as zeros
-        if (j + box_rows <= t.key_begin) return outside;
-        if ((unsigned)page >= (unsigned)p.pages) { report_bad_index(p); return outside; }
-        return page * p.page_size + (j - (int)p.page_div.div((uint32_t)j) * p.page_size);
-    };
-    auto load = [&] {                                          // the whole warp; false when the block gives up
-        if (g >= SLOTS) {                                      // the slot's last contents: keys are read out with their scores, values with their product
-            const int old = g - SLOTS, i = old >> 1;
-            if (!__all_sync(~0u, umma::mbar_wait((old & 1) ? &pv_done[i & 3] : &s_full[i & 3], (uint32_t)(i >> 2) & 1u, abort_flag))) return false;
-        }
-        const int boxes = __popc(__ballot_sync(~0u, box_row >= 0));
-        uint8_t* to = ring + load_slot * L::kSlotBytes;
-        const CUtensorMap* map = (g & 1) ? &v_map : &k_map;
-        const int batch = p.page_table ? 0 : t.seq;
-        if (umma::elect_one()) umma::mbar_expect_tx(&full[load_slot], (uint32_t)(boxes * box_rows) * 128u * DB);
-        __syncwarp();
-        for (int x = 0; x < boxes; x++) {
-            const int row = __shfl_sync(~0u, box_row, x);
-            if (umma::elect_one()) {
-                #pragma unroll
-                for (int b = 0; b < DB; b++) umma::tma_load_4d(to + b * (kStepKeys * 128) + x * box_rows * 128, map, &full[load_slot], b * 64, kv_head, row, batch);
-            }
-            __syncwarp();
-        }
-        if (g & 1) {
-            box_row = page_row(lo + (g >> 1) + 1, next_page);
-            next_page = fetch_page(lo + (g >> 1) + 2);
-        }
-        g++;
-        if (++load_slot == SLOTS) { load_slot = 0; load_phase ^= 1u; }
-        return true;
-    };
-    if (warp == 4) {
-        if (lane == 0) {
-            for (int s = 0; s < SLOTS; s++) umma::mbar_init(&full[s], 1);
-            for (int b = 0; b < 4; b++) { umma::mbar_init(&s_full[b], 1); umma::mbar_init(&pv_done[b], 1); }
-            for (int b = 0; b < 2; b++) umma::mbar_init(&p_ready[b], 128);
-            umma::mbar_init(&drained, 1);
-            abort_word = drain_word = 0;
-            umma::mbar_fence_init();
-        }
-        __syncwarp();
-        box_row = fetch_page(lo);
-        next_page = fetch_page(lo + 1);
-        box_row = page_row(lo, box_row);
-        while (g < 2 * n && g < SLOTS) load();
-    }
-
-    // queries and zeroed weights into shared memory, the N rows 128 bytes each, 16-byte pieces XORed with the row as the swizzle wants
-    for (int i = threadIdx.x; i < N * DB * 8; i += kStepThreads) {
-        const int r = i / (DB * 8), c = i - r * (DB * 8);
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < t.rows && c * 8 < p.dim) x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + row_offset(p, t, kv_head, t.row0 + r) + c * 8);
-        *reinterpret_cast<uint4*>(q_tile + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+    // the join may be scheduled onto the SMs as they drain; it waits for this grid before it reads
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < SLOTS; s++) umma::mbar_init(&full[s], 1);
+        for (int b = 0; b < 4; b++) { umma::mbar_init(&s_full[b], 1); umma::mbar_init(&pv_done[b], 1); }
+        for (int b = 0; b < 2; b++) { umma::mbar_init(&p_ready[b], 128); umma::mbar_init(&seg_full[b], 1); umma::mbar_init(&seg_empty[b], 6); }
+        umma::mbar_init(&drained, 1);
+        abort_word = drain_word = 0;
+        umma::mbar_fence_init();
     }
     if (threadIdx.x < N) fade[threadIdx.x] = 1.0f;            // of the columns that no row uses
-    for (int i = threadIdx.x; i < 2 * L::kPBytes / 16; i += kStepThreads) reinterpret_cast<uint4*>(p_tile)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x < N)
-        high[threadIdx.x] = p.page_table ? t.first_position + (int)p.group_div.div((uint32_t)(t.row0 + min((int)threadIdx.x, t.rows - 1))) + 1 : t.key_end;
-    umma::fence_proxy_async_smem();
+    if (warp == 4 && lane == 0) { umma::tma_prefetch_desc(&k_map); umma::tma_prefetch_desc(&v_map); }
+    if (warp == 5) umma::tmem_alloc(&tmem_slot, L::kColumns);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = tmem_slot, tmem_o = tmem + 2 * N;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, umma::mbar_wait(bar, parity, abort_flag)); };   // a whole warp
 
-    if (warp == 4) {
-        while (g < 2 * n && load()) {}
+    if (warp == 6) {
+        // ---- items: what this block works on, and its queries ---------------------------------------------------------------
+        const int total = total_units<N>(p);
+        const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+        const int x0 = min((int)blockIdx.x * share, total), x1 = min(x0 + share, total);
+        int x = x0, s = 0;
+        for (;; s++) {
+            const int buf = s & 1;
+            UnitPlace at = {};
+            Segment seg;
+            seg.n = -1;
+            int page = 0;
+            if (x < x1) {
+                at = place_unit<N>(p, x);
+                seg.t = row_tile_of<N>(p, at);
+                seg.kv_head = at.kv_head;
+                const int take = min(at.w.units - at.unit, x1 - x), first = first_tile_of(p, at);
+                // the units counted for the sequence may reach past the keys of this row tile
+                seg.lo = max(first + at.unit, seg.t.key_begin / kStepKeys);
+                const int hi = min(first + at.unit + take, (seg.t.key_end + kStepKeys - 1) / kStepKeys);
+                seg.n = seg.t.key_end > seg.t.key_begin ? max(hi - seg.lo, 0) : 0;
+                seg.part = at.unit == 0 && take == at.w.units ? -1 : (int)blockIdx.x * 2 + (x == x0 ? 0 : 1);
+                x += take;
+                const int j = seg.lo * kStepKeys + lane * box_rows;
+                if (p.page_table && seg.n > 0 && lane * box_rows < kStepKeys && j < seg.t.key_end && j + box_rows > seg.t.key_begin)
+                    page = p.page_table[(long long)seg.t.seq * p.table_width + (int)p.page_div.div((uint32_t)j)];
+            }
+            // sixteen-byte pieces of the rows, XORed with the row as the swizzle wants; loaded before the buffer is free
+            constexpr int PIECES = N * DB * 8 / 32;
+            constexpr int BATCH = PIECES < 16 ? PIECES : 16;
+            bool alive = true;
+            #pragma unroll 1
+            for (int base = 0; base < PIECES; base += BATCH) {
+                uint4 piece[BATCH];
+                #pragma unroll
+                for (int k = 0; k < BATCH; k++) {
+                    const int i = (base + k) * 32 + lane, r = i / (DB * 8), c = i - r * (DB * 8);
+                    piece[k] = make_uint4(0, 0, 0, 0);
+                    if (seg.n > 0 && r < seg.t.rows && c * 8 < p.dim)
+                        piece[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + row_offset(p, seg.t, seg.kv_head, seg.t.row0 + r) + c * 8);
+                }
+                if (base == 0 && s > 1) alive = wait(&seg_empty[buf], (uint32_t)((s >> 1) - 1) & 1u);
+                if (!alive) break;
+                uint8_t* q_tile = q_tiles + buf * L::kQBytes;
+                #pragma unroll
+                for (int k = 0; k < BATCH; k++) {
+                    const int i = (base + k) * 32 + lane, r = i / (DB * 8), c = i - r * (DB * 8);
+                    *reinterpret_cast<uint4*>(q_tile + (c >> 3) * (N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = piece[k];
+                }
+            }
+            if (!alive) break;
+            if (lane < 16) segments[buf].pages[lane] = page;
+            if (lane == 0) {
+                segments[buf].t = seg.t;
+                segments[buf].kv_head = seg.kv_head;
+                segments[buf].lo = seg.lo;
+                segments[buf].n = seg.n;
+                segments[buf].part = seg.part;
+            }
+            umma::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(&seg_full[buf]);
+            if (seg.n < 0) break;
+        }
+    } else if (warp == 4) {
+        // ---- copies: load number g is the keys (g even) or values (g odd) of this block's tile g / 2, into ring slot g % SLOTS ----------
+        int g = 0;
+        uint32_t slot = 0, phase = 0;
+        bool alive = true;
+        for (int s = 0; alive; s++) {
+            if (!wait(&seg_full[s & 1], (uint32_t)(s >> 1) & 1u)) break;
+            const Segment& seg = segments[s & 1];
+            const int n = seg.n, lo = seg.lo, key_begin = seg.t.key_begin, key_end = seg.t.key_end, kv_head = seg.kv_head, sequence = seg.t.seq;
+            const int batch = p.page_table ? 0 : sequence;
+            int page = seg.pages[lane & 15];
+            __syncwarp();
+            if (n < 0) break;
+            auto box_needed = [&](int j) { return lane * box_rows < kStepKeys && j < key_end; };
+            for (int i = 0; i < n && alive; i++) {
+                const int j = (lo + i) * kStepKeys + lane * box_rows;
+                int row = -1;                                  // cache row of this lane's box; -1: nothing to copy
+                if (box_needed(j)) {
+                    row = j;
+                    if (p.page_table) {
+                        row = p.pages * p.page_size;           // a row outside the map reads as zeros
+                        if (j + box_rows > key_begin) {        // pages in front of a window may be gone
+                            if ((unsigned)page < (unsigned)p.pages) row = page * p.page_size + (j - (int)p.page_div.div((uint32_t)j) * p.page_size);
+                            else report_bad_index(p);
+                        }
+                    }
+                }
+                // the next tile's pages, looked at when its turn comes: the copies never wait for the table
+                const int next_j = j + kStepKeys;
+                if (p.page_table && i + 1 < n && box_needed(next_j) && next_j + box_rows > key_begin)
+                    page = p.page_table[(long long)sequence * p.table_width + (int)p.page_div.div((uint32_t)next_j)];
+                const int boxes = __popc(__ballot_sync(~0u, row >= 0));
+                #pragma unroll 1
+                for (int kv = 0; kv < 2; kv++, g++) {
+                    if (g >= SLOTS) {                          // the slot's last contents: keys are read out with their scores, values with their product
+                        const int old = g - SLOTS, tile = old >> 1;
+                        if (!wait((old & 1) ? &pv_done[tile & 3] : &s_full[tile & 3], (uint32_t)(tile >> 2) & 1u)) { alive = false; break; }
+                    }
+                    uint8_t* to = ring + slot * L::kSlotBytes;
+                    const CUtensorMap* map = kv ? &v_map : &k_map;
+                    if (umma::elect_one()) umma::mbar_expect_tx(&full[slot], (uint32_t)(boxes * box_rows) * 128u * DB);
+                    __syncwarp();
+                    for (int x = 0; x < boxes; x++) {
+                        const int box_row = __shfl_sync(~0u, row, x);
+                        if (umma::elect_one()) {
+                            #pragma unroll
+                            for (int b = 0; b < DB; b++) umma::tma_load_4d(to + b * (kStepKeys * 128) + x * box_rows * 128, map, &full[slot], b * 64, kv_head, box_row, batch);
+                        }
+                        __syncwarp();
+                    }
+                    if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
+                }
+            }
+            if (lane == 0) umma::mbar_arrive(&seg_empty[s & 1]);
+        }
         if (lane == 0) {                                       // no copy of this block is in flight when it leaves
             for (int k = min(g, SLOTS); k > 0; k--) {
-                if (load_slot == 0) { load_slot = SLOTS; load_phase ^= 1u; }
-                load_slot--;
-                umma::mbar_wait(&full[load_slot], load_phase, &drain_word);
+                if (slot == 0) { slot = SLOTS; phase ^= 1u; }
+                slot--;
+                umma::mbar_wait(&full[slot], phase, &drain_word);
             }
         }
     } else if (warp == 5) {
-        // ---- products: the whole warp waits, one elected lane issues --------------------------------------------------------
+        // ---- products: the whole warp waits, one elected lane issues; the scores of the next tile, which may belong to the next item, go out before this
+        // tile's product with V, so that the softmax always has work -------------------------------------------------------------------
         constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t idesc_s = umma::instr_desc(fmt, fmt, 128, N), idesc_o = idesc_s | umma::kInstrAMnMajor;
         uint32_t slot = 0, phase = 0;
-        auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, umma::mbar_wait(bar, parity, abort_flag)); };
-        auto scores = [&](int i) {                             // S^T of tile i
-            if (!wait(&full[slot], phase)) return false;
+        auto step = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1u; } };
+        int s = -1, left = 0, tile = 0;                        // segment, tiles of it whose scores are still to come, number of the next tile
+        bool ok = true, fresh = false;
+        // advances to the next tile and issues its scores; false at the end (or when the block gives up: ok false)
+        auto scores = [&] {
+            fresh = false;
+            while (left == 0) {
+                s++;
+                if (!wait(&seg_full[s & 1], (uint32_t)(s >> 1) & 1u)) { ok = false; return false; }
+                left = segments[s & 1].n;
+                __syncwarp();
+                if (left < 0) return false;
+                fresh = true;
+                if (left == 0 && lane == 0) umma::mbar_arrive(&seg_empty[s & 1]);
+            }
+            if (!wait(&full[slot], phase)) { ok = false; return false; }
             umma::fence_after_sync();
-            const uint64_t da = umma::smem_desc_k_major_sw128(ring + slot * L::kSlotBytes), db = umma::smem_desc_k_major_sw128(q_tile);
+            left--;
+            const uint64_t da = umma::smem_desc_k_major_sw128(ring + slot * L::kSlotBytes), db = umma::smem_desc_k_major_sw128(q_tiles + (s & 1) * L::kQBytes);
             if (umma::elect_one()) {
                 #pragma unroll
                 for (int b = 0; b < DB; b++)
                     #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        umma::mma_ss<false>(tmem + (i & 1) * N, da + (uint64_t)(b * (kStepKeys * 128 >> 4) + 2 * k), db + (uint64_t)(b * (N * 128 >> 4) + 2 * k), idesc_s, (uint32_t)(b | k));
-                umma::mma_commit(&s_full[i & 3]);
+                        umma::mma_ss<false>(tmem + (tile & 1) * N, da + (uint64_t)(b * (kStepKeys * 128 >> 4) + 2 * k), db + (uint64_t)(b * (N * 128 >> 4) + 2 * k), idesc_s, (uint32_t)(b | k));
+                umma::mma_commit(&s_full[tile & 3]);
+                if (left == 0) umma::mma_commit(&seg_empty[s & 1]);      // the queries have been read
             }
             __syncwarp();
+            tile++;
+            step();                                            // on to this tile's values
             return true;
         };
-        auto step = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1u; } };
-        bool ok = n > 0 ? scores(0) : true;
-        for (int i = 0; i < n && ok; i++) {
-            step();                                            // this tile's values
+        bool more = scores();
+        while (more && ok) {
+            const int i = tile - 1;
+            const bool first = fresh;
             const uint32_t v_slot = slot, v_phase = phase;
-            step();                                            // the next tile's keys
-            ok = (i + 1 == n || scores(i + 1)) && wait(&p_ready[i & 1], (uint32_t)(i >> 1) & 1u) && wait(&full[v_slot], v_phase);
+            step();
+            more = scores();
+            if (!ok) break;
+            ok = wait(&p_ready[i & 1], (uint32_t)(i >> 1) & 1u) && wait(&full[v_slot], v_phase);
             if (!ok) break;
             umma::fence_after_sync();
             const uint64_t da = umma::smem_desc_mn_major_sw128(ring + v_slot * L::kSlotBytes, DB == 1 ? 0u : (uint32_t)(kStepKeys * 128));
@@ -241,7 +414,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                     #pragma unroll
                     for (int k = 0; k < 8; k++)
                         umma::mma_ss<false>(tmem_o + a * N, da + (uint64_t)(a * 2 * (kStepKeys * 128 >> 4) + k * (2048 >> 4)),
-                                            db + (uint64_t)((k >> 2) * (N * 128 >> 4) + 2 * (k & 3)), idesc_o, (uint32_t)(i | k));
+                                            db + (uint64_t)((k >> 2) * (N * 128 >> 4) + 2 * (k & 3)), idesc_o, first ? (uint32_t)k : 1u);
                 umma::mma_commit(&pv_done[i & 3]);
             }
             __syncwarp();
@@ -255,139 +428,174 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         // ---- softmax: a thread per key -------------------------------------------------------------------------------------
         const int key = threadIdx.x;
         const uint32_t lanes = (uint32_t)warp << 21;           // this warp's quarter of tensor memory
-        int all_high = t.key_end, all_low = 0;
-        if (p.page_table) {
-            all_high = high[0];
-            if (p.window > 0) all_low = high[N - 1] - p.window;
-        }
         const bool masked = p.mask_kind != kMaskNone;
-        float m[N], l[N];
-        #pragma unroll
-        for (int r = 0; r < N; r++) { m[r] = kNoMaximum; l[r] = 0.0f; }
         uint32_t slot = 0, phase = 0;
         bool ok = true;
-        for (int i = 0; i < n; i++) {
-            const int j0 = (lo + i) * kStepKeys, j = j0 + key;
-            if (++slot == SLOTS) { slot = 0; phase ^= 1u; }    // the slot of this tile's values
-            const bool edge = masked || j0 < all_low || j0 + kStepKeys > all_high;
-            bool dead = false;                                 // a key that no row sees: its value must not reach the product
-            float bias = 0.0f;
-            if (edge) {
-                dead = j >= t.key_end;
-                if (masked && !dead) { bias = key_bias(p, t.seq, j); dead = bias == -INFINITY; }
+        int i = 0;                                             // number of the tile
+        for (int s = 0; ok; s++) {
+            ok = umma::mbar_wait(&seg_full[s & 1], (uint32_t)(s >> 1) & 1u, abort_flag);
+            const Segment& seg = segments[s & 1];
+            const int n = seg.n;
+            if (any_of_softmax(!ok)) { ok = false; break; }
+            if (n < 0) break;
+            const int rows = seg.t.rows, key_end = seg.t.key_end, lo = seg.lo;
+            if (key < N) {
+                high[key] = p.page_table ? seg.t.first_position + (int)p.group_div.div((uint32_t)(seg.t.row0 + min(key, rows - 1))) + 1 : key_end;
+                top_of[key] = kNoMaximum;
             }
-            if (!umma::mbar_wait(&s_full[i & 3], (uint32_t)(i >> 2) & 1u, abort_flag)) ok = false;
-            umma::fence_after_sync();
-            float z[N];
-            tmem_load_columns<N>(tmem + lanes + (i & 1) * N, z);
-            float over = -INFINITY;
-            if (!edge) {
-                #pragma unroll
-                for (int c = 0; c < N; c += 4)
-                    if (c < t.rows)
-                        #pragma unroll
-                        for (int r = c; r < c + 4; r++) { z[r] *= p.scale_log2; over = fmaxf(over, z[r] - m[r]); }
-            } else {
-                #pragma unroll
-                for (int c = 0; c < N; c += 4)
-                    if (c < t.rows)
-                        #pragma unroll
-                        for (int r = c; r < c + 4; r++) {
-                            const bool seen = !dead && j < high[r] && (p.window == 0 || j >= high[r] - p.window);
-                            z[r] = seen ? __fmaf_rn(z[r], p.scale_log2, bias) : -INFINITY;
-                            over = fmaxf(over, z[r] - m[r]);
-                        }
+            softmax_sync();
+            int all_high = key_end, all_low = 0;
+            if (p.page_table) {
+                all_high = high[0];
+                if (p.window > 0) all_low = high[N - 1] - p.window;
             }
-            if (any_of_softmax(over > kMaximumSlack)) {
-                #pragma unroll
-                for (int c = 0; c < N; c += 4)
-                    if (c < t.rows)
-                        #pragma unroll
-                        for (int r = c; r < c + 4; r++) {
-                            float top = z[r];
-                            #pragma unroll
-                            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                            if (lane == 0) warp_top[warp][r] = top;
-                        }
-                softmax_sync();
-                #pragma unroll
-                for (int c = 0; c < N; c += 4)
-                    if (c < t.rows)
-                        #pragma unroll
-                        for (int r = c; r < c + 4; r++) {
-                            const float top = fmaxf(m[r], fmaxf(fmaxf(warp_top[0][r], warp_top[1][r]), fmaxf(warp_top[2][r], warp_top[3][r])));
-                            const float f = exp2_approx(m[r] - top);
-                            l[r] *= f;
-                            m[r] = top;
-                            if (key == r) fade[r] = f;
-                        }
-                softmax_sync();
-                if (i > 0) {
-                    if (!umma::mbar_wait(&pv_done[(i - 1) & 3], (uint32_t)((i - 1) >> 2) & 1u, abort_flag)) ok = false;
-                    umma::fence_after_sync();
-                    #pragma unroll
-                    for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<N>(tmem_o + lanes + a * N, fade);
+            float l[N];
+            #pragma unroll
+            for (int r = 0; r < N; r++) l[r] = 0.0f;
+            for (int it = 0; it < n; it++, i++) {
+                const int j0 = (lo + it) * kStepKeys, j = j0 + key;
+                if (++slot == SLOTS) { slot = 0; phase ^= 1u; }    // the slot of this tile's values
+                const bool edge = masked || j0 < all_low || j0 + kStepKeys > all_high;
+                bool dead = false;                             // a key that no row sees: its value must not reach the product
+                float bias = 0.0f;
+                if (edge) {
+                    dead = j >= key_end;
+                    if (masked && !dead) { bias = key_bias(p, seg.t.seq, j); dead = bias == -INFINITY; }
                 }
+                if (!umma::mbar_wait(&s_full[i & 3], (uint32_t)(i >> 2) & 1u, abort_flag)) ok = false;
+                umma::fence_after_sync();
+                float z[N];
+                __syncwarp();
+                tmem_load_columns<N>(tmem + lanes + (i & 1) * N, z);
+                float over = -INFINITY;
+                #pragma unroll
+                for (int c = 0; c < N; c += 4)
+                    if (c < rows) {
+                        const float4 m = *reinterpret_cast<const float4*>(top_of + c);
+                        const float mr[4] = {m.x, m.y, m.z, m.w};
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int r = c + e;
+                            if (!edge) z[r] *= p.scale_log2;
+                            else {
+                                const bool seen = !dead && j < high[r] && (p.window == 0 || j >= high[r] - p.window);
+                                z[r] = seen ? __fmaf_rn(z[r], p.scale_log2, bias) : -INFINITY;
+                            }
+                            over = fmaxf(over, z[r] - mr[e]);
+                        }
+                    }
+                if (any_of_softmax(over > kMaximumSlack || !ok)) {
+                    if (any_of_softmax(!ok)) { ok = false; break; }        // a wait has run out: all leave
+                    #pragma unroll
+                    for (int c = 0; c < N; c += 4)
+                        if (c < rows)
+                            #pragma unroll
+                            for (int r = c; r < c + 4; r++) {
+                                float top = z[r];
+                                #pragma unroll
+                                for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                                if (lane == 0) warp_top[warp][r] = top;
+                            }
+                    softmax_sync();
+                    if (key < N && (key & ~3) < rows) {
+                        const float old = top_of[key];
+                        const float top = fmaxf(old, fmaxf(fmaxf(warp_top[0][key], warp_top[1][key]), fmaxf(warp_top[2][key], warp_top[3][key])));
+                        fade[key] = exp2_approx(old - top);
+                        top_of[key] = top;
+                    }
+                    softmax_sync();
+                    #pragma unroll
+                    for (int c = 0; c < N; c += 4)
+                        if (c < rows) {
+                            const float4 f = *reinterpret_cast<const float4*>(fade + c);
+                            l[c] *= f.x; l[c + 1] *= f.y; l[c + 2] *= f.z; l[c + 3] *= f.w;
+                        }
+                    if (it > 0) {
+                        if (!umma::mbar_wait(&pv_done[(i - 1) & 3], (uint32_t)((i - 1) >> 2) & 1u, abort_flag)) ok = false;
+                        umma::fence_after_sync();
+                        __syncwarp();
+                        #pragma unroll
+                        for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<N>(tmem_o + lanes + a * N, fade);
+                    }
+                }
+                if (i > 1 && !umma::mbar_wait(&pv_done[(i - 2) & 3], (uint32_t)((i - 2) >> 2) & 1u, abort_flag)) ok = false;    // the weights of tile i - 2 are read
+                uint8_t* to = p_tile + (i & 1) * L::kPBytes + (key >> 6) * (N * 128) + (key & 7) * 2;
+                #pragma unroll
+                for (int c = 0; c < N; c += 4)
+                    if (c < rows) {
+                        const float4 m = *reinterpret_cast<const float4*>(top_of + c);
+                        const float mr[4] = {m.x, m.y, m.z, m.w};
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int r = c + e;
+                            const float w = exp2_approx(z[r] - mr[e]);
+                            l[r] += w;
+                            *reinterpret_cast<T*>(to + r * 128 + ((((key & 63) >> 3) ^ (r & 7)) << 4)) = from_float<T>(w);
+                        }
+                    }
+                if (dead) {                                    // a weight of zero times a NaN would still be one
+                    if (!umma::mbar_wait(&full[slot], phase, abort_flag)) ok = false;
+                    uint8_t* row = ring + slot * L::kSlotBytes + key * 128;
+                    #pragma unroll
+                    for (int b = 0; b < DB; b++)
+                        #pragma unroll
+                        for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(row + b * (kStepKeys * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+                }
+                umma::fence_proxy_async_smem();
+                umma::fence_before_sync();
+                umma::mbar_arrive(&p_ready[i & 1]);
+                if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
             }
-            if (i > 1 && !umma::mbar_wait(&pv_done[(i - 2) & 3], (uint32_t)((i - 2) >> 2) & 1u, abort_flag)) ok = false;    // the weights of tile i - 2 are read
-            uint8_t* to = p_tile + (i & 1) * L::kPBytes + (key >> 6) * (N * 128) + (key & 7) * 2;
+            if (any_of_softmax(!ok)) { ok = false; break; }
+            // the item's (or its part's) result
+            if (n > 0) {
+                if (!umma::mbar_wait(&pv_done[(i - 1) & 3], (uint32_t)((i - 1) >> 2) & 1u, abort_flag)) ok = false;
+                umma::fence_after_sync();
+            }
+            __syncwarp();
+            float x[L::kOAccs][N];
+            #pragma unroll
+            for (int a = 0; a < L::kOAccs; a++) tmem_load_columns<N>(tmem_o + lanes + a * N, x[a]);
+            // sums of weights over the keys, through the idle weight buffers: [row][key] as floats
+            float* turn = reinterpret_cast<float*>(p_tile);
             #pragma unroll
             for (int c = 0; c < N; c += 4)
-                if (c < t.rows)
+                if (c < rows)
                     #pragma unroll
-                    for (int r = c; r < c + 4; r++) {
-                        const float w = exp2_approx(z[r] - m[r]);
-                        l[r] += w;
-                        *reinterpret_cast<T*>(to + r * 128 + ((((key & 63) >> 3) ^ (r & 7)) << 4)) = from_float<T>(w);
-                    }
-            if (dead) {                                        // a weight of zero times a NaN would still be one
-                if (!umma::mbar_wait(&full[slot], phase, abort_flag)) ok = false;
-                uint8_t* row = ring + slot * L::kSlotBytes + key * 128;
-                #pragma unroll
-                for (int b = 0; b < DB; b++)
-                    #pragma unroll
-                    for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(row + b * (kStepKeys * 128) + c * 16) = make_uint4(0, 0, 0, 0);
-            }
-            umma::fence_proxy_async_smem();
-            umma::fence_before_sync();
-            umma::mbar_arrive(&p_ready[i & 1]);
-            if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
-            if (!ok) break;
-        }
-        if (n > 0) {
-            if (ok) ok = umma::mbar_wait(&pv_done[(n - 1) & 3], (uint32_t)((n - 1) >> 2) & 1u, abort_flag);
-            umma::fence_after_sync();
-        }
-        // o[r][d] into the ring (everything in it has been read), the sums of weights across the keys
-        float* o = reinterpret_cast<float*>(ring);
-        __syncwarp();
-        if (n > 0) {
-            #pragma unroll
-            for (int a = 0; a < L::kOAccs; a++) {
-                float x[N];
-                tmem_load_columns<N>(tmem_o + lanes + a * N, x);
-                const int d = a * 128 + key;
-                if (d < DB * 64)
-                    #pragma unroll
-                    for (int r = 0; r < N; r++) if (r < t.rows) o[r * L::kPitch + d] = x[r];
-            }
-        }
-        #pragma unroll
-        for (int r = 0; r < N; r++) {
-            if (r < t.rows) {
-                float sum = l[r];
+                    for (int r = c; r < c + 4; r++) turn[r * 128 + key] = l[r];
+            softmax_sync();
+            for (int r = warp; r < rows; r += 4) {
+                float sum = (turn[r * 128 + lane] + turn[r * 128 + 32 + lane]) + (turn[r * 128 + 64 + lane] + turn[r * 128 + 96 + lane]);
                 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-                if (lane == 0) warp_sum[warp][r] = sum;
+                if (lane == 0) {
+                    sums[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    if (seg.part >= 0) part_stats[(long long)seg.part * N + r] = make_float2(sum == 0.0f ? -INFINITY : top_of[r], sum);
+                }
             }
+            softmax_sync();
+            if (seg.part >= 0) {
+                #pragma unroll
+                for (int a = 0; a < L::kOAccs; a++) {
+                    const int d = a * 128 + key;
+                    if (d < L::kDims)
+                        #pragma unroll
+                        for (int r = 0; r < N; r++) if (r < rows) part_o[((long long)seg.part * N + r) * L::kDims + d] = x[a][r];
+                }
+            } else {
+                #pragma unroll
+                for (int a = 0; a < L::kOAccs; a++) {
+                    const int d = a * 128 + key;
+                    if (d < p.dim)
+                        #pragma unroll
+                        for (int r = 0; r < N; r++)
+                            if (r < rows) reinterpret_cast<T*>(p.y)[row_offset(p, seg.t, seg.kv_head, seg.t.row0 + r) + d] = from_float<T>(sums[r] == 0.0f ? 0.0f : x[a][r] * sums[r]);
+                }
+            }
+            umma::fence_before_sync();
+            softmax_sync();                                    // sums, weights and the segment have been read by all
+            if (lane == 0) umma::mbar_arrive(&seg_empty[s & 1]);
         }
-        softmax_sync();
-        #pragma unroll
-        for (int r = 0; r < N; r++)
-            if (key == r && r < t.rows) {
-                const float sum = (warp_sum[0][r] + warp_sum[1][r]) + (warp_sum[2][r] + warp_sum[3][r]);
-                stats[r] = make_float2(sum == 0.0f ? -INFINITY : m[r], sum);
-            }
     }
     umma::fence_before_sync();
     __syncthreads();
@@ -396,31 +604,141 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         umma::fence_after_sync();
         umma::tmem_dealloc(tmem, L::kColumns);
     }
-    join_and_store<T, L::kPitch, kStepThreads>(p, t, kv_head, reinterpret_cast<const float*>(ring), stats);
+}
+
+// Joins the partial results of the items that several blocks of the kernel above share.  Block (c, q): the item that begins in share c and ends behind it, four
+// of its rows; its parts lie in slot 2 c (or 2 c + 1) and in the first slots of the shares behind.  Eight warps take every eighth part each.
+constexpr int kStepJoinThreads = 256;
+template <typename T, int N, int DIMS>
+__global__ void __launch_bounds__(kStepJoinThreads) attention_step_join(const __grid_constant__ AttentionProblem p, const float* __restrict__ part_o, const float2* __restrict__ part_stats) {
+    constexpr int WARPS = kStepJoinThreads / 32, QUADS = DIMS / 4, PER_LANE = (QUADS + 31) / 32;
+    __shared__ float4 partial[WARPS][QUADS];
+    __shared__ float partial_l[WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int total = total_units<N>(p);
+    const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x, c = blockIdx.x;
+    const int x0 = min(c * share, total), x1 = min(x0 + share, total);
+    UnitPlace at = {};
+    bool mine = x1 > x0;
+    int begin = 0, end = 0;
+    if (mine) {
+        at = place_unit<N>(p, x1 - 1);
+        begin = x1 - 1 - at.unit;
+        end = begin + at.w.units;
+        mine = begin >= x0 && end > x1;
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!mine) return;
+    const RowTile t = row_tile_of<N>(p, at);
+    const int parts = (end - 1) / share - c + 1;
+    auto slot = [&](int k) { return k == 0 ? 2 * c + (begin == x0 ? 0 : 1) : 2 * (c + k); };
+    const bool aligned = (p.dim & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
+    for (int r = blockIdx.y * 4; r < min((int)blockIdx.y * 4 + 4, t.rows); r++) {
+        float top = -INFINITY;
+        for (int k = lane; k < parts; k += 32) top = fmaxf(top, part_stats[(long long)slot(k) * N + r].x);
+        #pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        float l = 0.0f;
+        float4 sum[PER_LANE];
+        #pragma unroll
+        for (int e = 0; e < PER_LANE; e++) sum[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        #pragma unroll 4
+        for (int k = warp; k < parts; k += WARPS) {
+            const long long row = (long long)slot(k) * N + r;
+            const float2 s = part_stats[row];
+            const float w = partial_weight(s.x, top);
+            if (s.x != -INFINITY) l = __fmaf_rn(s.y, w, l);
+            #pragma unroll
+            for (int e = 0; e < PER_LANE; e++) {
+                const int quad = lane + e * 32;
+                if (quad < QUADS) {
+                    const float4 v = *reinterpret_cast<const float4*>(part_o + row * DIMS + quad * 4);
+                    if (s.x != -INFINITY) {                    // a part without a key holds nothing
+                        sum[e].x = __fmaf_rn(v.x, w, sum[e].x); sum[e].y = __fmaf_rn(v.y, w, sum[e].y);
+                        sum[e].z = __fmaf_rn(v.z, w, sum[e].z); sum[e].w = __fmaf_rn(v.w, w, sum[e].w);
+                    }
+                }
+            }
+        }
+        #pragma unroll
+        for (int e = 0; e < PER_LANE; e++) if (lane + e * 32 < QUADS) partial[warp][lane + e * 32] = sum[e];
+        if (lane == 0) partial_l[warp] = l;
+        __syncthreads();
+        for (int quad = threadIdx.x; quad < QUADS; quad += kStepJoinThreads) {
+            float all = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float4 v = partial[w][quad];
+                all += partial_l[w];
+                x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+            }
+            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) x[e] *= inv;
+            if (quad * 4 < p.dim) store4(reinterpret_cast<T*>(p.y) + row_offset(p, t, at.kv_head, t.row0 + r) + quad * 4, x, p.dim - quad * 4, aligned);
+        }
+        __syncthreads();
+    }
 }
 
 template <typename T, int DB, int N, int SLOTS> static bool launch_step(const AttentionProblem& p) {
     using L = StepLayout<DB, N, SLOTS>;
+    DeviceState* st = acquire_device();
+    if (!st) return false;
     int box_rows = cache_box_rows(p);
     CUtensorMap k_map, v_map;
     if (!make_cache_map(&k_map, p, p.k, box_rows) || !make_cache_map(&v_map, p, p.v, box_rows)) {
         set_error(TOPS_ERR_CUDA, "attention_step: the tensor map was refused");
         return false;
     }
-    int tiles = (int)attention_tiles(p, N);
-    const int splits = attention_splits(p, tiles, 8 * kNumSMs, kStepKeys);
+    const void* kernel = (const void*)attention_step_kernel<T, DB, N, SLOTS>;
+    if (!ensure_dynamic_smem(kernel, L::kSmem)) return false;
+    // as many blocks as the SMs hold, but none that cannot get a tile
+    const long long tiles = attention_tiles(p, N) * p.kv_heads * ((p.keys + kStepKeys - 1) / kStepKeys);
+    const int per_sm = 2 * (L::kSmem + 3072) <= 228 * 1024 ? 2 : 1;
+    const int blocks = (int)(tiles < (long long)st->sm_count * per_sm ? tiles : (long long)st->sm_count * per_sm);
+    cudaStream_t stream = current_stream();
+    const size_t o_bytes = (size_t)2 * blocks * N * L::kDims * sizeof(float), stat_bytes = (size_t)2 * blocks * N * sizeof(float2);
+    void* scratch = nullptr;
+    if (!TOPS_CUDA_OK(cudaMallocAsync(&scratch, o_bytes + stat_bytes, stream))) return false;
+    float* part_o = reinterpret_cast<float*>(scratch);
+    float2* part_stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + o_bytes);
     AttentionProblem copy = p;
-    void* args[] = {&k_map, &v_map, &copy, &tiles, &box_rows};
-    if (!launch_attention((const void*)attention_step_kernel<T, DB, N, SLOTS>, p, N, kStepThreads, L::kSmem, splits, args, "attention_step")) return false;
-    count_tensor_core_launch();
-    return true;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kStepThreads);
+    cfg.dynamicSmemBytes = L::kSmem;
+    cfg.stream = stream;
+    void* args[] = {&k_map, &v_map, &copy, &box_rows, &part_o, &part_stats};
+    bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_step");
+    if (ok) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t join = {};
+        join.gridDim = dim3((unsigned)blocks, N / 4);
+        join.blockDim = dim3(kStepJoinThreads);
+        join.stream = stream;
+        join.attrs = attr;
+        join.numAttrs = 1;
+        void* join_args[] = {&copy, &part_o, &part_stats};
+        ok = check_cuda(cudaLaunchKernelExC(&join, (const void*)attention_step_join<T, N, L::kDims>, join_args), "attention_step_join");
+    }
+    ok = TOPS_CUDA_OK(cudaFreeAsync(scratch, stream)) && ok;
+    if (ok) count_tensor_core_launch();
+    return ok;
 }
 
 template <typename T> static bool launch_step_size(const AttentionProblem& p) {
     const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
-    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 6>(p) : rows <= 32 ? launch_step<T, 1, 32, 6>(p) : launch_step<T, 1, 64, 8>(p);
-    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 3>(p) : rows <= 32 ? launch_step<T, 2, 32, 5>(p) : launch_step<T, 2, 64, 5>(p);
+    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 6>(p) : rows <= 32 ? launch_step<T, 1, 32, 5>(p) : launch_step<T, 1, 64, 7>(p);
+    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 3>(p) : rows <= 32 ? launch_step<T, 2, 32, 5>(p) : launch_step<T, 2, 64, 4>(p);
     return rows <= 16 ? launch_step<T, 4, 16, 3>(p) : launch_step<T, 4, 32, 2>(p);
+}
+
+// The units of the whole problem are counted in 32 bits.
+bool attention_step_fits(const AttentionProblem& p) {
+    return attention_tiles(p, 16) * p.kv_heads * ((p.keys + kStepKeys - 1) / kStepKeys + 1) < 0x40000000ll;
 }
 
 bool attention_step(const AttentionProblem& p) {
