@@ -19,8 +19,9 @@
 // second small kernel joins them in the order of the keys.  (Clusters that join through distributed shared memory were measured first: the GPU
 // holds only 15 clusters of eight such blocks at a time, 120 of 148 SMs, and 16 items then took two rounds: 235 us where this takes REPLACE_LONG.)
 //
-// Warps 0-3 softmax, warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs, warp 6 finds the next item and brings
-// its queries.
+// Warps 0-3 and 8-11: two softmax groups that take the items in turn -- one finishes its item (sums, tensor memory, stores) while the other
+// is in the next item's tiles.  Warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs, warp 6 finds the next
+// item and brings its queries.
 #include "attention_common.cuh"
 
 #include <type_traits>
@@ -29,7 +30,7 @@ namespace tops {
 
 void count_tensor_core_launch();
 
-constexpr int kStepThreads = 224;
+constexpr int kStepThreads = 384;
 constexpr int kStepKeys = 128;
 
 template <int DB, int N, int SLOTS> struct StepLayout {
@@ -39,7 +40,7 @@ template <int DB, int N, int SLOTS> struct StepLayout {
     static constexpr int kDims = DB * 64;
     static constexpr int kSmem = SLOTS * kSlotBytes + 2 * kQBytes + 2 * kPBytes + 1024;   // and room to align
     static constexpr int kOAccs = DB > 2 ? 2 : 1;             // accumulators of 128 dimensions
-    static constexpr uint32_t kColumns = (2 + kOAccs) * N <= 64 ? 64 : (2 + kOAccs) * N <= 128 ? 128 : 256;
+    static constexpr uint32_t kUsed = (2 + 2 * kOAccs) * N, kColumns = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
     static_assert(SLOTS <= 8, "a slot's release is read from barriers of the last four tiles");
 };
 
@@ -48,7 +49,7 @@ template <int DB, int N, int SLOTS> struct StepLayout {
 // rows without a key are visited as well).
 struct SequenceWork { int start, tokens, length, units, row_tiles; };
 
-template <int N> __device__ __forceinline__ SequenceWork sequence_work(const AttentionProblem& p, int b) {
+template <int N> __device__ __forceinline__ SequenceWork sequence_work(const AttentionProblem& p, int b, bool whole) {
     SequenceWork w = {0, 0, 0, 0, 0};
     if (b >= p.batch) return w;
     int first_key = 0;
@@ -65,7 +66,7 @@ template <int N> __device__ __forceinline__ SequenceWork sequence_work(const Att
         w.length = p.kv_length ? min(max(p.kv_length[b], 0), p.keys) : p.keys;
     }
     w.row_tiles = (w.tokens * p.group + N - 1) / N;
-    w.units = max(1, (w.length + kStepKeys - 1) / kStepKeys - first_key / kStepKeys);
+    w.units = whole ? 1 : max(1, (w.length + kStepKeys - 1) / kStepKeys - first_key / kStepKeys);
     return w;
 }
 
@@ -73,10 +74,10 @@ template <int N> __device__ __forceinline__ SequenceWork sequence_work(const Att
 struct UnitPlace { SequenceWork w; int seq, row_tile, kv_head, unit; };
 
 // All units; called by whole warps.
-template <int N> __device__ __forceinline__ int total_units(const AttentionProblem& p) {
+template <int N> __device__ __forceinline__ int total_units(const AttentionProblem& p, bool whole) {
     int sum = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
-        const SequenceWork w = sequence_work<N>(p, b);
+        const SequenceWork w = sequence_work<N>(p, b, whole);
         sum += w.row_tiles * w.units;
     }
     #pragma unroll
@@ -84,12 +85,12 @@ template <int N> __device__ __forceinline__ int total_units(const AttentionProbl
     return sum * p.kv_heads;
 }
 
-template <int N> __device__ __forceinline__ UnitPlace place_unit(const AttentionProblem& p, int x) {
+template <int N> __device__ __forceinline__ UnitPlace place_unit(const AttentionProblem& p, int x, bool whole) {
     const int lane = threadIdx.x & 31;
     UnitPlace at = {};
     int before = 0;
     for (int base = 0; base < p.batch; base += 32) {
-        const SequenceWork w = sequence_work<N>(p, base + lane);
+        const SequenceWork w = sequence_work<N>(p, base + lane, whole);
         const int mine = w.row_tiles * w.units * p.kv_heads;
         int sum = mine;
         #pragma unroll
@@ -146,15 +147,15 @@ struct Segment {
     int pages[16];               // pages of tile lo
 };
 
-// True for all 128 softmax threads if it is for one.
-__device__ __forceinline__ bool any_of_softmax(bool x) {
+// True for all 128 threads of a softmax group if it is for one.
+__device__ __forceinline__ bool any_of_softmax(int group, bool x) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
-        "barrier.cta.red.or.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"((uint32_t)x) : "memory");
+        "barrier.cta.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"((uint32_t)x), "r"(1 + group) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync(int group) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory"); }
 
 template <int N> __device__ __forceinline__ void tmem_load_columns(uint32_t at, float (&x)[N]) {
     if constexpr (N == 16) {
@@ -198,31 +199,33 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                       const __grid_constant__ AttentionProblem p, const int box_rows, float* __restrict__ part_o, float2* __restrict__ part_stats) {
     using L = StepLayout<DB, N, SLOTS>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], seg_full[2], seg_empty[2], drained;
+    __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], seg_full[2], seg_empty[2], o_full[2], turn[2], drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word, drain_word;
     __shared__ __align__(16) unsigned char segment_memory[2 * sizeof(Segment)];
     Segment* segments = reinterpret_cast<Segment*>(segment_memory);
-    __shared__ __align__(16) float warp_top[4][N], fade[N], top_of[N], sums[N];
-    __shared__ int high[N];
+    __shared__ __align__(16) float group_floats[2][7 * N];    // per softmax group: warp_top[4], fade, top_of, sums
+    __shared__ int group_high[2][N];
     uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_tiles = ring + SLOTS * L::kSlotBytes;
     uint8_t* p_tile = q_tiles + 2 * L::kQBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort_flag = &abort_word;
 
-    // the join may be scheduled onto the SMs as they drain; it waits for this grid before it reads
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; s++) umma::mbar_init(&full[s], 1);
         for (int b = 0; b < 4; b++) { umma::mbar_init(&s_full[b], 1); umma::mbar_init(&pv_done[b], 1); }
-        for (int b = 0; b < 2; b++) { umma::mbar_init(&p_ready[b], 128); umma::mbar_init(&seg_full[b], 1); umma::mbar_init(&seg_empty[b], 6); }
+        for (int b = 0; b < 2; b++) { umma::mbar_init(&p_ready[b], 128); umma::mbar_init(&seg_full[b], 1); umma::mbar_init(&seg_empty[b], 7); umma::mbar_init(&o_full[b], 1); umma::mbar_init(&turn[b], 4); }
         umma::mbar_init(&drained, 1);
         abort_word = drain_word = 0;
         umma::mbar_fence_init();
     }
-    if (threadIdx.x < N) fade[threadIdx.x] = 1.0f;            // of the columns that no row uses
+    if (threadIdx.x < 2 * N) group_floats[threadIdx.x / N][4 * N + threadIdx.x % N] = 1.0f;      // fade of the columns that no row uses
     if (warp == 4 && lane == 0) { umma::tma_prefetch_desc(&k_map); umma::tma_prefetch_desc(&v_map); }
+    // Scheduled while the previous kernel of the stream drains; nothing so far has touched global or tensor memory.  The join in turn may be scheduled early: it
+    // waits for this grid before it reads.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 5) umma::tmem_alloc(&tmem_slot, L::kColumns);
     umma::fence_before_sync();
     __syncthreads();
@@ -232,7 +235,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
 
     if (warp == 6) {
         // ---- items: what this block works on, and its queries ---------------------------------------------------------------
-        const int total = total_units<N>(p);
+        const bool whole = part_o == nullptr;                  // the unit is the item: nothing is split, nothing joined
+        const int total = total_units<N>(p, whole);
         const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
         const int x0 = min((int)blockIdx.x * share, total), x1 = min(x0 + share, total);
         int x = x0, s = 0;
@@ -243,13 +247,13 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             seg.n = -1;
             int page = 0;
             if (x < x1) {
-                at = place_unit<N>(p, x);
+                at = place_unit<N>(p, x, whole);
                 seg.t = row_tile_of<N>(p, at);
                 seg.kv_head = at.kv_head;
                 const int take = min(at.w.units - at.unit, x1 - x), first = first_tile_of(p, at);
                 // the units counted for the sequence may reach past the keys of this row tile
                 seg.lo = max(first + at.unit, seg.t.key_begin / kStepKeys);
-                const int hi = min(first + at.unit + take, (seg.t.key_end + kStepKeys - 1) / kStepKeys);
+                const int all = (seg.t.key_end + kStepKeys - 1) / kStepKeys, hi = whole ? all : min(first + at.unit + take, all);
                 seg.n = seg.t.key_end > seg.t.key_begin ? max(hi - seg.lo, 0) : 0;
                 seg.part = at.unit == 0 && take == at.w.units ? -1 : (int)blockIdx.x * 2 + (x == x0 ? 0 : 1);
                 x += take;
@@ -399,6 +403,9 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         while (more && ok) {
             const int i = tile - 1;
             const bool first = fresh;
+            const uint32_t o_at = tmem_o + (uint32_t)((s & 1) * L::kOAccs * N);
+            const int of = s;
+            const bool last = left == 0;
             const uint32_t v_slot = slot, v_phase = phase;
             step();
             more = scores();
@@ -413,9 +420,10 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 for (int a = 0; a < L::kOAccs; a++)
                     #pragma unroll
                     for (int k = 0; k < 8; k++)
-                        umma::mma_ss<false>(tmem_o + a * N, da + (uint64_t)(a * 2 * (kStepKeys * 128 >> 4) + k * (2048 >> 4)),
+                        umma::mma_ss<false>(o_at + a * N, da + (uint64_t)(a * 2 * (kStepKeys * 128 >> 4) + k * (2048 >> 4)),
                                             db + (uint64_t)((k >> 2) * (N * 128 >> 4) + 2 * (k & 3)), idesc_o, first ? (uint32_t)k : 1u);
                 umma::mma_commit(&pv_done[i & 3]);
+                if (last) umma::mma_commit(&o_full[of & 1]);   // a barrier of its own: the other group's tiles may be far ahead when this one is looked at
             }
             __syncwarp();
         }
@@ -424,26 +432,42 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             __syncwarp();
             umma::mbar_wait(&drained, 0, &drain_word);
         }
-    } else {
+    } else if (warp != 7) {
         // ---- softmax: a thread per key -------------------------------------------------------------------------------------
-        const int key = threadIdx.x;
-        const uint32_t lanes = (uint32_t)warp << 21;           // this warp's quarter of tensor memory
+        const int group = warp >> 3, quarter = warp & 3, key = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)quarter << 21;        // this warp's quarter of tensor memory
+        float (*warp_top)[N] = reinterpret_cast<float (*)[N]>(group_floats[group]);
+        float *fade = group_floats[group] + 4 * N, *top_of = fade + N, *sums = top_of + N;
+        int* high = group_high[group];
         const bool masked = p.mask_kind != kMaskNone;
-        uint32_t slot = 0, phase = 0;
+        uint32_t slot = 0, phase = 0, o_phase = 0;             // o_phase counts this group's items that had a key
         bool ok = true;
         int i = 0;                                             // number of the tile
-        for (int s = 0; ok; s++) {
+        for (int s = 0;; s++) {
+            if (any_of_softmax(group, !ok)) break;
             ok = umma::mbar_wait(&seg_full[s & 1], (uint32_t)(s >> 1) & 1u, abort_flag);
             const Segment& seg = segments[s & 1];
             const int n = seg.n;
-            if (any_of_softmax(!ok)) { ok = false; break; }
+            const uint32_t my_o = tmem_o + lanes + (uint32_t)((s & 1) * L::kOAccs * N);
+            if (any_of_softmax(group, !ok)) { ok = false; break; }
             if (n < 0) break;
+            if ((s & 1) != group) {                            // the other group's item: only the ring and the tile count move on
+                i += n;
+                const uint32_t moved = slot + 2u * (uint32_t)n;
+                slot = moved % SLOTS;
+                phase ^= (moved / SLOTS) & 1u;
+                softmax_sync(group);                           // all have read n
+                if (key == 0) umma::mbar_arrive(&seg_empty[s & 1]);
+                // and this group's tiles begin when the other's end: barriers that count tiles tell two neighbouring phases apart, no more
+                ok = umma::mbar_wait(&turn[s & 1], (uint32_t)(s >> 1) & 1u, abort_flag);
+                continue;
+            }
             const int rows = seg.t.rows, key_end = seg.t.key_end, lo = seg.lo;
             if (key < N) {
                 high[key] = p.page_table ? seg.t.first_position + (int)p.group_div.div((uint32_t)(seg.t.row0 + min(key, rows - 1))) + 1 : key_end;
                 top_of[key] = kNoMaximum;
             }
-            softmax_sync();
+            softmax_sync(group);
             int all_high = key_end, all_low = 0;
             if (p.page_table) {
                 all_high = high[0];
@@ -484,8 +508,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                             over = fmaxf(over, z[r] - mr[e]);
                         }
                     }
-                if (any_of_softmax(over > kMaximumSlack || !ok)) {
-                    if (any_of_softmax(!ok)) { ok = false; break; }        // a wait has run out: all leave
+                if (any_of_softmax(group, over > kMaximumSlack || !ok)) {
+                    if (any_of_softmax(group, !ok)) { ok = false; break; }        // a wait has run out: all leave
                     #pragma unroll
                     for (int c = 0; c < N; c += 4)
                         if (c < rows)
@@ -494,16 +518,16 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                                 float top = z[r];
                                 #pragma unroll
                                 for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                                if (lane == 0) warp_top[warp][r] = top;
+                                if (lane == 0) warp_top[quarter][r] = top;
                             }
-                    softmax_sync();
+                    softmax_sync(group);
                     if (key < N && (key & ~3) < rows) {
                         const float old = top_of[key];
                         const float top = fmaxf(old, fmaxf(fmaxf(warp_top[0][key], warp_top[1][key]), fmaxf(warp_top[2][key], warp_top[3][key])));
                         fade[key] = exp2_approx(old - top);
                         top_of[key] = top;
                     }
-                    softmax_sync();
+                    softmax_sync(group);
                     #pragma unroll
                     for (int c = 0; c < N; c += 4)
                         if (c < rows) {
@@ -515,7 +539,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                         umma::fence_after_sync();
                         __syncwarp();
                         #pragma unroll
-                        for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<N>(tmem_o + lanes + a * N, fade);
+                        for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<N>(my_o + a * N, fade);
                     }
                 }
                 if (i > 1 && !umma::mbar_wait(&pv_done[(i - 2) & 3], (uint32_t)((i - 2) >> 2) & 1u, abort_flag)) ok = false;    // the weights of tile i - 2 are read
@@ -546,34 +570,36 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 umma::mbar_arrive(&p_ready[i & 1]);
                 if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
             }
-            if (any_of_softmax(!ok)) { ok = false; break; }
+            if (any_of_softmax(group, !ok)) { ok = false; break; }
+            if (lane == 0) umma::mbar_arrive(&turn[s & 1]);
             // the item's (or its part's) result
             if (n > 0) {
-                if (!umma::mbar_wait(&pv_done[(i - 1) & 3], (uint32_t)((i - 1) >> 2) & 1u, abort_flag)) ok = false;
+                if (!umma::mbar_wait(&o_full[group], o_phase, abort_flag)) ok = false;
                 umma::fence_after_sync();
+                o_phase ^= 1u;
             }
             __syncwarp();
             float x[L::kOAccs][N];
             #pragma unroll
-            for (int a = 0; a < L::kOAccs; a++) tmem_load_columns<N>(tmem_o + lanes + a * N, x[a]);
-            // sums of weights over the keys, through the idle weight buffers: [row][key] as floats
-            float* turn = reinterpret_cast<float*>(p_tile);
+            for (int a = 0; a < L::kOAccs; a++) tmem_load_columns<N>(my_o + a * N, x[a]);
+            // sums of weights over the keys
             #pragma unroll
             for (int c = 0; c < N; c += 4)
                 if (c < rows)
                     #pragma unroll
-                    for (int r = c; r < c + 4; r++) turn[r * 128 + key] = l[r];
-            softmax_sync();
-            for (int r = warp; r < rows; r += 4) {
-                float sum = (turn[r * 128 + lane] + turn[r * 128 + 32 + lane]) + (turn[r * 128 + 64 + lane] + turn[r * 128 + 96 + lane]);
-                #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-                if (lane == 0) {
-                    sums[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    if (seg.part >= 0) part_stats[(long long)seg.part * N + r] = make_float2(sum == 0.0f ? -INFINITY : top_of[r], sum);
-                }
+                    for (int r = c; r < c + 4; r++) {
+                        float sum = l[r];
+                        #pragma unroll
+                        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+                        if (lane == 0) warp_top[quarter][r] = sum;
+                    }
+            softmax_sync(group);
+            if (key < rows) {
+                const float sum = (warp_top[0][key] + warp_top[1][key]) + (warp_top[2][key] + warp_top[3][key]);
+                sums[key] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (seg.part >= 0) part_stats[(long long)seg.part * N + key] = make_float2(sum == 0.0f ? -INFINITY : top_of[key], sum);
             }
-            softmax_sync();
+            softmax_sync(group);
             if (seg.part >= 0) {
                 #pragma unroll
                 for (int a = 0; a < L::kOAccs; a++) {
@@ -593,7 +619,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 }
             }
             umma::fence_before_sync();
-            softmax_sync();                                    // sums, weights and the segment have been read by all
+            softmax_sync(group);                                    // sums, weights and the segment have been read by all
             if (lane == 0) umma::mbar_arrive(&seg_empty[s & 1]);
         }
     }
@@ -615,14 +641,14 @@ __global__ void __launch_bounds__(kStepJoinThreads) attention_step_join(const __
     __shared__ float4 partial[WARPS][QUADS];
     __shared__ float partial_l[WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int total = total_units<N>(p);
+    const int total = total_units<N>(p, false);
     const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x, c = blockIdx.x;
     const int x0 = min(c * share, total), x1 = min(x0 + share, total);
     UnitPlace at = {};
     bool mine = x1 > x0;
     int begin = 0, end = 0;
     if (mine) {
-        at = place_unit<N>(p, x1 - 1);
+        at = place_unit<N>(p, x1 - 1, false);
         begin = x1 - 1 - at.unit;
         end = begin + at.w.units;
         mine = begin >= x0 && end > x1;
@@ -693,46 +719,53 @@ template <typename T, int DB, int N, int SLOTS> static bool launch_step(const At
     }
     const void* kernel = (const void*)attention_step_kernel<T, DB, N, SLOTS>;
     if (!ensure_dynamic_smem(kernel, L::kSmem)) return false;
-    // as many blocks as the SMs hold, but none that cannot get a tile
-    const long long tiles = attention_tiles(p, N) * p.kv_heads * ((p.keys + kStepKeys - 1) / kStepKeys);
-    const int per_sm = 2 * (L::kSmem + 3072) <= 228 * 1024 ? 2 : 1;
-    const int blocks = (int)(tiles < (long long)st->sm_count * per_sm ? tiles : (long long)st->sm_count * per_sm);
+    // One block per SM (two of the small ones: with heads of 64 a tile is half as long to copy but not to work on), but none that cannot get a tile.  Where an item cannot have more than four tiles (512 keys), a block takes it whole: the join costs as much as
+    // three tiles in a row.
+    const long long units = (p.keys + kStepKeys - 1) / kStepKeys, items = attention_tiles(p, N) * p.kv_heads;
+    const bool whole = units <= 4;
+    const long long most = whole ? items : items * units;
+    const long long room = (long long)st->sm_count * (DB == 1 && N == 16 ? 2 : 1);
+    const int blocks = (int)(most < room ? most : room);
     cudaStream_t stream = current_stream();
     const size_t o_bytes = (size_t)2 * blocks * N * L::kDims * sizeof(float), stat_bytes = (size_t)2 * blocks * N * sizeof(float2);
     void* scratch = nullptr;
-    if (!TOPS_CUDA_OK(cudaMallocAsync(&scratch, o_bytes + stat_bytes, stream))) return false;
+    if (!whole && !TOPS_CUDA_OK(cudaMallocAsync(&scratch, o_bytes + stat_bytes, stream))) return false;
     float* part_o = reinterpret_cast<float*>(scratch);
-    float2* part_stats = reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + o_bytes);
+    float2* part_stats = whole ? nullptr : reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + o_bytes);
     AttentionProblem copy = p;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kStepThreads);
     cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     void* args[] = {&k_map, &v_map, &copy, &box_rows, &part_o, &part_stats};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_step");
-    if (ok) {
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t join = {};
-        join.gridDim = dim3((unsigned)blocks, N / 4);
-        join.blockDim = dim3(kStepJoinThreads);
-        join.stream = stream;
-        join.attrs = attr;
-        join.numAttrs = 1;
-        void* join_args[] = {&copy, &part_o, &part_stats};
-        ok = check_cuda(cudaLaunchKernelExC(&join, (const void*)attention_step_join<T, N, L::kDims>, join_args), "attention_step_join");
+    if (!whole) {
+        if (ok) {
+            cudaLaunchConfig_t join = {};
+            join.gridDim = dim3((unsigned)blocks, N / 4);
+            join.blockDim = dim3(kStepJoinThreads);
+            join.stream = stream;
+            join.attrs = attr;
+            join.numAttrs = 1;
+            void* join_args[] = {&copy, &part_o, &part_stats};
+            ok = check_cuda(cudaLaunchKernelExC(&join, (const void*)attention_step_join<T, N, L::kDims>, join_args), "attention_step_join");
+        }
+        ok = TOPS_CUDA_OK(cudaFreeAsync(scratch, stream)) && ok;
     }
-    ok = TOPS_CUDA_OK(cudaFreeAsync(scratch, stream)) && ok;
     if (ok) count_tensor_core_launch();
     return ok;
 }
 
 template <typename T> static bool launch_step_size(const AttentionProblem& p) {
     const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
-    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 6>(p) : rows <= 32 ? launch_step<T, 1, 32, 5>(p) : launch_step<T, 1, 64, 7>(p);
-    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 3>(p) : rows <= 32 ? launch_step<T, 2, 32, 5>(p) : launch_step<T, 2, 64, 4>(p);
+    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 5>(p) : rows <= 32 ? launch_step<T, 1, 32, 5>(p) : launch_step<T, 1, 64, 7>(p);
+    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 5>(p) : rows <= 32 ? launch_step<T, 2, 32, 5>(p) : launch_step<T, 2, 64, 4>(p);
     return rows <= 16 ? launch_step<T, 4, 16, 3>(p) : launch_step<T, 4, 32, 2>(p);
 }
 

@@ -100,9 +100,9 @@ class Paged:
             k, v = exact(rng, (length, kv_heads, dim), dtype, spread), exact(rng, (length, kv_heads, dim), dtype)
             self.keys.append(k)
             self.values.append(v)
-            for j in range(length):
-                self.key_cache[mine[j // page], j % page] = k[j]
-                self.value_cache[mine[j // page], j % page] = v[j]
+            j = np.arange(length)
+            self.key_cache[mine[j // page], j % page] = k
+            self.value_cache[mine[j // page], j % page] = v
         self.query_start = np.concatenate([[0], np.cumsum([n for n, _ in pairs])]).astype(np.int32)
         self.kv_length = np.array([length for _, length in pairs], np.int32)
 

@@ -81,6 +81,16 @@ def test_rows_behind_the_last_sequence_stay(dtype, tokens):
     assert np.all(got[2 * tokens:] == 7.0)
 
 
+def test_many_tiles_per_block():
+    """Long enough that every block works through tens of 128-key tiles of one item and goes on to the next."""
+    problem = Paged(_rng("many tiles"), "bfloat16", 4, 2, 64, 128, [(1, 70001), (3, 60011), (1, 65)])
+    want, tol = problem.want()
+    assert_close(run_paged(problem), want, tol)
+    problem = Paged(_rng("many tiles", 128), "float16", 1, 1, 128, 64, [(1, 200003)])
+    want, tol = problem.want()
+    assert_close(run_paged(problem), want, tol)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tokens", [1, 200])
 def test_large_scores(dtype, tokens):
