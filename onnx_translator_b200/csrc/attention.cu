@@ -67,6 +67,7 @@ bool make_cache_map(CUtensorMap* map, const AttentionProblem& p, const void* bas
 static bool run_attention(const AttentionProblem& p) {
     if (whole_pieces(p)) {
         const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
+        if (rows > 64 && attention_chunk_takes(p)) return attention_chunk(p);
         if (cache_box_rows(p) > 0 && rows <= 64 && attention_step_fits(p)) return attention_step(p);
         return attention_rows(p);
     }

@@ -292,6 +292,8 @@ bool make_cache_map(CUtensorMap* map, const AttentionProblem& p, const void* bas
 // Rows of a box that stay inside a page (dense: 128): a divisor of 128 that is a multiple of the 8-row swizzle group; 0 if there is none.
 int cache_box_rows(const AttentionProblem& p);
 
+bool attention_chunk_takes(const AttentionProblem& p);
+bool attention_chunk(const AttentionProblem& p);     // 16-bit types, dim <= 128, cache_box_rows > 0, scale > 0: 256 rows per block, tcgen05
 bool attention_step_fits(const AttentionProblem& p);
 bool attention_step(const AttentionProblem& p);      // 16-bit types, cache_box_rows > 0: up to 64 rows per block, tcgen05
 bool attention_fma(const AttentionProblem& p);       // any type, any dim up to 256

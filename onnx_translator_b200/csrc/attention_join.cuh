@@ -1,0 +1,117 @@
+// Items that several blocks share: where the partial results lie, and the kernel that joins them.
+//
+// Block c of the main kernel works on the c-th share of all work; slot 2 c holds the partial result of its first item, slot 2 c + 1 that of its last one.
+// An item that begins in share c and ends in share c + k - 1 has its k parts in c's slot and in slots 2 (c + 1), 2 (c + 2), ...: block c leaves a
+// job that says so.  The parts are joined in the order of the keys, so the result does not depend on timing.
+#pragma once
+
+#include "attention_common.cuh"
+
+namespace tops {
+
+struct JoinJob {
+    RowTile t;
+    int kv_head = 0;
+    int parts = 0;               // 0: no item of this share goes on in the next
+    int slot = 0;                // of the first part
+};
+
+struct PartialResults {          // scratch of one call, from the stream-ordered pool
+    float* o = nullptr;          // [2 * blocks][N][DIMS]
+    float2* stats = nullptr;     // [2 * blocks][N]: maximum, sum of weights
+    JoinJob* jobs = nullptr;     // [blocks]
+};
+
+inline bool allocate_partials(PartialResults& parts, int blocks, int rows, int dims, cudaStream_t stream) {
+    const size_t o_bytes = (size_t)2 * blocks * rows * dims * sizeof(float), stat_bytes = (size_t)2 * blocks * rows * sizeof(float2);
+    char* scratch = nullptr;
+    if (!TOPS_CUDA_OK(cudaMallocAsync((void**)&scratch, o_bytes + stat_bytes + (size_t)blocks * sizeof(JoinJob), stream))) return false;
+    parts.o = reinterpret_cast<float*>(scratch);
+    parts.stats = reinterpret_cast<float2*>(scratch + o_bytes);
+    parts.jobs = reinterpret_cast<JoinJob*>(scratch + o_bytes + stat_bytes);
+    return true;
+}
+
+// Block (c, q): four rows of job c.  Eight warps take every eighth part each.
+constexpr int kJoinThreads = 256;
+template <typename T, int N, int DIMS>
+__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttentionProblem p, const PartialResults parts) {
+    constexpr int WARPS = kJoinThreads / 32, QUADS = DIMS / 4, PER_LANE = (QUADS + 31) / 32;
+    __shared__ float4 partial[WARPS][QUADS];
+    __shared__ float partial_l[WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const JoinJob job = parts.jobs[blockIdx.x];
+    if (job.parts == 0 || (int)blockIdx.y * 4 >= job.t.rows) return;
+    auto slot = [&](int k) { return k == 0 ? job.slot : 2 * ((int)blockIdx.x + k); };
+    const bool aligned = (p.dim & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
+    for (int r = blockIdx.y * 4; r < min((int)blockIdx.y * 4 + 4, job.t.rows); r++) {
+        float top = -INFINITY;
+        for (int k = lane; k < job.parts; k += 32) top = fmaxf(top, parts.stats[(long long)slot(k) * N + r].x);
+        #pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        float l = 0.0f;
+        float4 sum[PER_LANE];
+        #pragma unroll
+        for (int e = 0; e < PER_LANE; e++) sum[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        #pragma unroll 4
+        for (int k = warp; k < job.parts; k += WARPS) {
+            const long long row = (long long)slot(k) * N + r;
+            const float2 s = parts.stats[row];
+            const float w = partial_weight(s.x, top);
+            if (s.x != -INFINITY) l = __fmaf_rn(s.y, w, l);
+            #pragma unroll
+            for (int e = 0; e < PER_LANE; e++) {
+                const int quad = lane + e * 32;
+                if (quad < QUADS) {
+                    const float4 v = *reinterpret_cast<const float4*>(parts.o + row * DIMS + quad * 4);
+                    if (s.x != -INFINITY) {                    // a part without a key holds nothing
+                        sum[e].x = __fmaf_rn(v.x, w, sum[e].x); sum[e].y = __fmaf_rn(v.y, w, sum[e].y);
+                        sum[e].z = __fmaf_rn(v.z, w, sum[e].z); sum[e].w = __fmaf_rn(v.w, w, sum[e].w);
+                    }
+                }
+            }
+        }
+        #pragma unroll
+        for (int e = 0; e < PER_LANE; e++) if (lane + e * 32 < QUADS) partial[warp][lane + e * 32] = sum[e];
+        if (lane == 0) partial_l[warp] = l;
+        __syncthreads();
+        for (int quad = threadIdx.x; quad < QUADS; quad += kJoinThreads) {
+            float all = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float4 v = partial[w][quad];
+                all += partial_l[w];
+                x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+            }
+            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+            #pragma unroll
+            for (int e = 0; e < 4; e++) x[e] *= inv;
+            if (quad * 4 < p.dim) store4(reinterpret_cast<T*>(p.y) + row_offset(p, job.t, job.kv_head, job.t.row0 + r) + quad * 4, x, p.dim - quad * 4, aligned);
+        }
+        __syncthreads();
+    }
+}
+
+// Enqueues the join (when the main kernel was launched: `ok`) and gives the scratch back in stream order.
+template <typename T, int N, int DIMS>
+bool join_partials(const AttentionProblem& p, const PartialResults& parts, int blocks, cudaStream_t stream, bool ok) {
+    if (ok) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)blocks, N / 4);
+        cfg.blockDim = dim3(kJoinThreads);
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        AttentionProblem copy = p;
+        PartialResults copy_parts = parts;
+        void* args[] = {&copy, &copy_parts};
+        ok = check_cuda(cudaLaunchKernelExC(&cfg, (const void*)attention_join<T, N, DIMS>, args), "attention_join");
+    }
+    return TOPS_CUDA_OK(cudaFreeAsync(parts.o, stream)) && ok;
+}
+
+}  // namespace tops

@@ -22,7 +22,7 @@
 // Warps 0-3 and 8-11: two softmax groups that take the items in turn -- one finishes its item (sums, tensor memory, stores) while the other
 // is in the next item's tiles.  Warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs, warp 6 finds the next
 // item and brings its queries.
-#include "attention_common.cuh"
+#include "attention_join.cuh"
 
 #include <type_traits>
 
@@ -196,7 +196,7 @@ constexpr float kMaximumSlack = 8.0f;
 template <typename T, int DB, int N, int SLOTS>
 __global__ void __launch_bounds__(kStepThreads)
 attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                      const __grid_constant__ AttentionProblem p, const int box_rows, float* __restrict__ part_o, float2* __restrict__ part_stats) {
+                      const __grid_constant__ AttentionProblem p, const int box_rows, const PartialResults parts) {
     using L = StepLayout<DB, N, SLOTS>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], seg_full[2], seg_empty[2], o_full[2], turn[2], drained;
@@ -235,11 +235,12 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
 
     if (warp == 6) {
         // ---- items: what this block works on, and its queries ---------------------------------------------------------------
-        const bool whole = part_o == nullptr;                  // the unit is the item: nothing is split, nothing joined
+        const bool whole = parts.o == nullptr;                 // the unit is the item: nothing is split, nothing joined
         const int total = total_units<N>(p, whole);
         const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
         const int x0 = min((int)blockIdx.x * share, total), x1 = min(x0 + share, total);
         int x = x0, s = 0;
+        JoinJob job;                                           // the item that begins in this share and ends behind it
         for (;; s++) {
             const int buf = s & 1;
             UnitPlace at = {};
@@ -256,6 +257,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 const int all = (seg.t.key_end + kStepKeys - 1) / kStepKeys, hi = whole ? all : min(first + at.unit + take, all);
                 seg.n = seg.t.key_end > seg.t.key_begin ? max(hi - seg.lo, 0) : 0;
                 seg.part = at.unit == 0 && take == at.w.units ? -1 : (int)blockIdx.x * 2 + (x == x0 ? 0 : 1);
+                if (seg.part >= 0 && x - at.unit >= x0 && x - at.unit + at.w.units > x1)
+                    job = JoinJob{seg.t, seg.kv_head, (x - at.unit + at.w.units - 1) / share - (int)blockIdx.x + 1, seg.part};
                 x += take;
                 const int j = seg.lo * kStepKeys + lane * box_rows;
                 if (p.page_table && seg.n > 0 && lane * box_rows < kStepKeys && j < seg.t.key_end && j + box_rows > seg.t.key_begin)
@@ -298,6 +301,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             if (lane == 0) umma::mbar_arrive(&seg_full[buf]);
             if (seg.n < 0) break;
         }
+        if (!whole && lane == 0) parts.jobs[blockIdx.x] = job;
     } else if (warp == 4) {
         // ---- copies: load number g is the keys (g even) or values (g odd) of this block's tile g / 2, into ring slot g % SLOTS ----------
         int g = 0;
@@ -597,7 +601,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             if (key < rows) {
                 const float sum = (warp_top[0][key] + warp_top[1][key]) + (warp_top[2][key] + warp_top[3][key]);
                 sums[key] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (seg.part >= 0) part_stats[(long long)seg.part * N + key] = make_float2(sum == 0.0f ? -INFINITY : top_of[key], sum);
+                if (seg.part >= 0) parts.stats[(long long)seg.part * N + key] = make_float2(sum == 0.0f ? -INFINITY : top_of[key], sum);
             }
             softmax_sync(group);
             if (seg.part >= 0) {
@@ -606,7 +610,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                     const int d = a * 128 + key;
                     if (d < L::kDims)
                         #pragma unroll
-                        for (int r = 0; r < N; r++) if (r < rows) part_o[((long long)seg.part * N + r) * L::kDims + d] = x[a][r];
+                        for (int r = 0; r < N; r++) if (r < rows) parts.o[((long long)seg.part * N + r) * L::kDims + d] = x[a][r];
                 }
             } else {
                 #pragma unroll
@@ -632,81 +636,6 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     }
 }
 
-// Joins the partial results of the items that several blocks of the kernel above share.  Block (c, q): the item that begins in share c and ends behind it, four
-// of its rows; its parts lie in slot 2 c (or 2 c + 1) and in the first slots of the shares behind.  Eight warps take every eighth part each.
-constexpr int kStepJoinThreads = 256;
-template <typename T, int N, int DIMS>
-__global__ void __launch_bounds__(kStepJoinThreads) attention_step_join(const __grid_constant__ AttentionProblem p, const float* __restrict__ part_o, const float2* __restrict__ part_stats) {
-    constexpr int WARPS = kStepJoinThreads / 32, QUADS = DIMS / 4, PER_LANE = (QUADS + 31) / 32;
-    __shared__ float4 partial[WARPS][QUADS];
-    __shared__ float partial_l[WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int total = total_units<N>(p, false);
-    const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x, c = blockIdx.x;
-    const int x0 = min(c * share, total), x1 = min(x0 + share, total);
-    UnitPlace at = {};
-    bool mine = x1 > x0;
-    int begin = 0, end = 0;
-    if (mine) {
-        at = place_unit<N>(p, x1 - 1, false);
-        begin = x1 - 1 - at.unit;
-        end = begin + at.w.units;
-        mine = begin >= x0 && end > x1;
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!mine) return;
-    const RowTile t = row_tile_of<N>(p, at);
-    const int parts = (end - 1) / share - c + 1;
-    auto slot = [&](int k) { return k == 0 ? 2 * c + (begin == x0 ? 0 : 1) : 2 * (c + k); };
-    const bool aligned = (p.dim & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
-    for (int r = blockIdx.y * 4; r < min((int)blockIdx.y * 4 + 4, t.rows); r++) {
-        float top = -INFINITY;
-        for (int k = lane; k < parts; k += 32) top = fmaxf(top, part_stats[(long long)slot(k) * N + r].x);
-        #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        float l = 0.0f;
-        float4 sum[PER_LANE];
-        #pragma unroll
-        for (int e = 0; e < PER_LANE; e++) sum[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        #pragma unroll 4
-        for (int k = warp; k < parts; k += WARPS) {
-            const long long row = (long long)slot(k) * N + r;
-            const float2 s = part_stats[row];
-            const float w = partial_weight(s.x, top);
-            if (s.x != -INFINITY) l = __fmaf_rn(s.y, w, l);
-            #pragma unroll
-            for (int e = 0; e < PER_LANE; e++) {
-                const int quad = lane + e * 32;
-                if (quad < QUADS) {
-                    const float4 v = *reinterpret_cast<const float4*>(part_o + row * DIMS + quad * 4);
-                    if (s.x != -INFINITY) {                    // a part without a key holds nothing
-                        sum[e].x = __fmaf_rn(v.x, w, sum[e].x); sum[e].y = __fmaf_rn(v.y, w, sum[e].y);
-                        sum[e].z = __fmaf_rn(v.z, w, sum[e].z); sum[e].w = __fmaf_rn(v.w, w, sum[e].w);
-                    }
-                }
-            }
-        }
-        #pragma unroll
-        for (int e = 0; e < PER_LANE; e++) if (lane + e * 32 < QUADS) partial[warp][lane + e * 32] = sum[e];
-        if (lane == 0) partial_l[warp] = l;
-        __syncthreads();
-        for (int quad = threadIdx.x; quad < QUADS; quad += kStepJoinThreads) {
-            float all = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            #pragma unroll
-            for (int w = 0; w < WARPS; w++) {
-                const float4 v = partial[w][quad];
-                all += partial_l[w];
-                x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
-            }
-            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-            #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] *= inv;
-            if (quad * 4 < p.dim) store4(reinterpret_cast<T*>(p.y) + row_offset(p, t, at.kv_head, t.row0 + r) + quad * 4, x, p.dim - quad * 4, aligned);
-        }
-        __syncthreads();
-    }
-}
-
 template <typename T, int DB, int N, int SLOTS> static bool launch_step(const AttentionProblem& p) {
     using L = StepLayout<DB, N, SLOTS>;
     DeviceState* st = acquire_device();
@@ -727,11 +656,8 @@ template <typename T, int DB, int N, int SLOTS> static bool launch_step(const At
     const long long room = (long long)st->sm_count * (DB == 1 && N == 16 ? 2 : 1);
     const int blocks = (int)(most < room ? most : room);
     cudaStream_t stream = current_stream();
-    const size_t o_bytes = (size_t)2 * blocks * N * L::kDims * sizeof(float), stat_bytes = (size_t)2 * blocks * N * sizeof(float2);
-    void* scratch = nullptr;
-    if (!whole && !TOPS_CUDA_OK(cudaMallocAsync(&scratch, o_bytes + stat_bytes, stream))) return false;
-    float* part_o = reinterpret_cast<float*>(scratch);
-    float2* part_stats = whole ? nullptr : reinterpret_cast<float2*>(reinterpret_cast<char*>(scratch) + o_bytes);
+    PartialResults parts;
+    if (!whole && !allocate_partials(parts, blocks, N, L::kDims, stream)) return false;
     AttentionProblem copy = p;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -743,21 +669,9 @@ template <typename T, int DB, int N, int SLOTS> static bool launch_step(const At
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    void* args[] = {&k_map, &v_map, &copy, &box_rows, &part_o, &part_stats};
+    void* args[] = {&k_map, &v_map, &copy, &box_rows, &parts};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_step");
-    if (!whole) {
-        if (ok) {
-            cudaLaunchConfig_t join = {};
-            join.gridDim = dim3((unsigned)blocks, N / 4);
-            join.blockDim = dim3(kStepJoinThreads);
-            join.stream = stream;
-            join.attrs = attr;
-            join.numAttrs = 1;
-            void* join_args[] = {&copy, &part_o, &part_stats};
-            ok = check_cuda(cudaLaunchKernelExC(&join, (const void*)attention_step_join<T, N, L::kDims>, join_args), "attention_step_join");
-        }
-        ok = TOPS_CUDA_OK(cudaFreeAsync(scratch, stream)) && ok;
-    }
+    if (!whole) ok = join_partials<T, N, L::kDims>(copy, parts, blocks, stream, ok);
     if (ok) count_tensor_core_launch();
     return ok;
 }
