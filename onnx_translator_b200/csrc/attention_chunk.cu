@@ -35,8 +35,10 @@ template <int DB, int SLOTS> struct ChunkLayout {
 };
 
 // ---- the row of all items ------------------------------------------------------------------------------------------------
-// Sequence b has `count` items per key head; item i weighs base + slope * (i + 1) -- about the keys it sees; exactness only matters for the balance.
+// Sequence b has `count` items per key head; item i weighs base + slope * (i + 1): the keys it sees and kItemKeys for what an item costs besides
+// (fetching queries, filling the pipeline, storing: as long as 400 keys, measured on items of 12 tiles).  Exactness only matters for the balance.
 // All weights of a sequence have a closed sum, so a place in the row is found without walking the items.
+constexpr int kItemKeys = 448;
 struct ChunkSequence { int start, tokens, length, count, base, slope; };
 
 __device__ __forceinline__ ChunkSequence chunk_sequence(const AttentionProblem& p, int b, int item_tokens) {
@@ -56,6 +58,7 @@ __device__ __forceinline__ ChunkSequence chunk_sequence(const AttentionProblem& 
         w.length = p.kv_length ? min(max(p.kv_length[b], 0), p.keys) : p.keys;
         w.base = max(1, w.length);
     }
+    w.base += kItemKeys;
     w.count = (w.tokens + item_tokens - 1) / item_tokens;
     return w;
 }
@@ -216,7 +219,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     const int first = seg.t.key_begin / kChunkKeys;
                     const int all = seg.t.key_end > seg.t.key_begin ? (seg.t.key_end + kChunkKeys - 1) / kChunkKeys - first : 0;
                     // a place inside the item's weight as a number of its tiles; the item's end is all of them
-                    auto tiles_at = [&](long long o) { return o >= at.weight ? all : (int)min((long long)all, (o + kChunkKeys - 1) / kChunkKeys); };
+                    auto tiles_at = [&](long long o) { return o >= at.weight ? all : (int)min((long long)all, max(o - kItemKeys + kChunkKeys - 1, 0ll) / kChunkKeys); };
                     const int from = tiles_at(at.offset), to = tiles_at(at.offset + take);
                     seg.lo = first + from;
                     seg.n = to - from;
@@ -396,7 +399,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         const int group = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)quarter << 21;        // this warp's quarter of tensor memory
         const uint32_t s_at = tmem + lanes + group * 128, o_at = tmem + lanes + 256 + group * 128;
-        const float scale = p.scale_log2;
+        const float scale = p.scale_log2, per_scale = 1.0f / p.scale_log2;
         uint32_t slot = 0, phase = 0;                          // of the ring, both row tiles use every tile of keys
         uint32_t mine = 0, items = 0;                          // tiles of scores and items of this row tile so far
         bool ok = true;
@@ -424,21 +427,25 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 all_high = __reduce_min_sync(~0u, high);
                 if (p.window > 0) { low = high - p.window; all_low = __reduce_max_sync(~0u, low); }
             }
-            float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;          // m in units of the raw score (masked: of log2)
+            float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;          // m in units of the raw score
             for (int i = 0; i < n; i++) {
                 const int j0 = (lo + i) * kChunkKeys;
                 if (++slot == SLOTS) { slot = 0; phase ^= 1u; }    // the slot of this tile's values
                 bool dead = j0 + row >= t.key_end;             // a key that no row sees: its value must not reach the product
+                bool biased = false;
                 if constexpr (MASKED) {
                     __syncwarp();                              // the last tile's biases have been read
+                    bool some = false;
                     #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int j = j0 + e * 32 + lane;
                         const float b = j < t.key_end ? key_bias(p, t.seq, j) : -INFINITY;
-                        warp_bias[warp][e * 32 + lane] = b;
+                        warp_bias[warp][e * 32 + lane] = b * per_scale;       // in units of the raw score
+                        some = some || b != 0.0f;
                         if (e == quarter) dead = b == -INFINITY;
                     }
                     __syncwarp();
+                    biased = __any_sync(~0u, some);
                 }
                 ok = wait(&s_full[group], mine & 1u);
                 if (!ok) break;
@@ -447,15 +454,16 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 #pragma unroll
                 for (int c = 0; c < 128; c += 32) umma::tmem_load_32x32(s_at + c, *reinterpret_cast<uint32_t (*)[32]>(x + c));
                 umma::tmem_load_wait();
-                if constexpr (MASKED) {
+                if (MASKED && biased) {
                     #pragma unroll
                     for (int c = 0; c < 128; c += 4) {
                         const float4 b = *reinterpret_cast<const float4*>(&warp_bias[warp][c]);
                         const float bias[4] = {b.x, b.y, b.z, b.w};
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) x[c + e] = bias[e] == -INFINITY ? -INFINITY : __fmaf_rn(x[c + e], scale, bias[e]);
+                        for (int e = 0; e < 4; e++) x[c + e] = bias[e] == -INFINITY ? -INFINITY : x[c + e] + bias[e];
                     }
-                } else if (j0 < all_low || j0 + kChunkKeys > all_high) {
+                }
+                if (!MASKED && (j0 < all_low || j0 + kChunkKeys > all_high)) {
                     const int to = high - j0, from = low - j0;
                     #pragma unroll
                     for (int c = 0; c < 128; c++) x[c] = c < to && c >= from ? x[c] : -INFINITY;
@@ -466,10 +474,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     #pragma unroll
                     for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], fmaxf(x[c + 2 * e], x[c + 2 * e + 1]));
                 const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float unit = MASKED ? 1.0f : scale;
-                if (__any_sync(~0u, valid && (most - m) * unit > kChunkSlack)) {
+                if (__any_sync(~0u, valid && (most - m) * scale > kChunkSlack)) {
                     const float next = fmaxf(m, most);
-                    const float f = m == -INFINITY ? 0.0f : exp2_approx((m - next) * unit);
+                    const float f = m == -INFINITY ? 0.0f : exp2_approx((m - next) * scale);
                     m = next;
                     l0 *= f; l1 *= f;
                     if (i > 0) {
@@ -487,14 +494,14 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : -m * unit;
+                const float base = m == -INFINITY ? 0.0f : -m * scale;
                 #pragma unroll
                 for (int c = 0; c < 128; c += 64) {
                     uint32_t w[32];
                     #pragma unroll
                     for (int e = 0; e < 64; e += 2) {
                         float &a = x[c + e], &b = x[c + e + 1];
-                        fma2(a, b, unit, base);
+                        fma2(a, b, scale, base);
                         a = exp2_approx(a);
                         b = exp2_approx(b);
                         add2(l0, l1, a, b);
@@ -530,7 +537,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 umma::fence_after_sync();
             }
             if (part >= 0) {
-                if (valid) parts.stats[(long long)part * kChunkRows + r] = make_float2(l == 0.0f ? -INFINITY : MASKED ? m : m * scale, l);
+                if (valid) parts.stats[(long long)part * kChunkRows + r] = make_float2(l == 0.0f ? -INFINITY : m * scale, l);
                 float* to = parts.o + ((long long)part * kChunkRows + r) * L::kDims;
                 #pragma unroll 1
                 for (int c = 0; c < L::kDims; c += 32) {
@@ -616,9 +623,10 @@ template <typename T, int DB, int SLOTS> static bool launch_chunk(const Attentio
     return ok;
 }
 
-// A whole group of heads has to fit a tile, and the scores' maximum is taken before they are scaled: the scale has to be positive.
+// A whole group of heads has to fit a tile.  Maximum and mask are applied to the scores before they are scaled: the scale has to be positive, and not
+// so small that a mask divided by it overflows.
 bool attention_chunk_takes(const AttentionProblem& p) {
-    return p.dim <= 128 && p.group <= 128 && p.scale_log2 > 0.0f && cache_box_rows(p) > 0;
+    return p.dim <= 128 && p.group <= 128 && p.scale_log2 > (p.mask_kind == kMaskNone ? 0.0f : 1e-4f) && cache_box_rows(p) > 0;
 }
 
 bool attention_chunk(const AttentionProblem& p) {

@@ -32,9 +32,10 @@ inline bool allocate_partials(PartialResults& parts, int blocks, int rows, int d
     return true;
 }
 
-// Block (c, q): four rows of job c.  Eight warps take every eighth part each.
+// Block (c, q): ROWS rows of job c, eight warps.  With few parts a warp joins whole rows by itself, all loads in flight together; with many (a few long sequences
+// over all SMs) the warps take every eighth part of a row and meet in shared memory.
 constexpr int kJoinThreads = 256;
-template <typename T, int N, int DIMS>
+template <typename T, int N, int DIMS, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttentionProblem p, const PartialResults parts) {
     constexpr int WARPS = kJoinThreads / 32, QUADS = DIMS / 4, PER_LANE = (QUADS + 31) / 32;
     __shared__ float4 partial[WARPS][QUADS];
@@ -42,10 +43,51 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const JoinJob job = parts.jobs[blockIdx.x];
-    if (job.parts == 0 || (int)blockIdx.y * 4 >= job.t.rows) return;
+    const int row_begin = (int)blockIdx.y * ROWS, row_end = min(row_begin + ROWS, job.t.rows);
+    if (job.parts == 0 || row_begin >= row_end) return;
     auto slot = [&](int k) { return k == 0 ? job.slot : 2 * ((int)blockIdx.x + k); };
     const bool aligned = (p.dim & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
-    for (int r = blockIdx.y * 4; r < min((int)blockIdx.y * 4 + 4, job.t.rows); r++) {
+    if (job.parts <= 8) {
+        #pragma unroll 1
+        for (int r = row_begin + warp; r < row_end; r += WARPS) {
+            float2 s = make_float2(-INFINITY, 0.0f);
+            if (lane < job.parts) s = parts.stats[(long long)slot(lane) * N + r];
+            float4 v[8][PER_LANE];
+            #pragma unroll
+            for (int k = 0; k < 8; k++)
+                #pragma unroll
+                for (int e = 0; e < PER_LANE; e++)
+                    if (k < job.parts && lane + e * 32 < QUADS) v[k][e] = *reinterpret_cast<const float4*>(parts.o + ((long long)slot(k) * N + r) * DIMS + (lane + e * 32) * 4);
+            const float top = fmaxf(fmaxf(fmaxf(__shfl_sync(~0u, s.x, 0), __shfl_sync(~0u, s.x, 1)), fmaxf(__shfl_sync(~0u, s.x, 2), __shfl_sync(~0u, s.x, 3))),
+                                    fmaxf(fmaxf(__shfl_sync(~0u, s.x, 4), __shfl_sync(~0u, s.x, 5)), fmaxf(__shfl_sync(~0u, s.x, 6), __shfl_sync(~0u, s.x, 7))));
+            const float w = partial_weight(s.x, top), weighted = s.x == -INFINITY ? 0.0f : s.y * w;
+            float l = 0.0f;
+            float x[PER_LANE][4] = {};
+            #pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float wk = __shfl_sync(~0u, w, k), mk = __shfl_sync(~0u, s.x, k);
+                l += __shfl_sync(~0u, weighted, k);
+                if (k < job.parts && mk != -INFINITY)          // a part without a key holds nothing
+                    #pragma unroll
+                    for (int e = 0; e < PER_LANE; e++) {
+                        if (lane + e * 32 >= QUADS) continue;
+                        x[e][0] = __fmaf_rn(v[k][e].x, wk, x[e][0]); x[e][1] = __fmaf_rn(v[k][e].y, wk, x[e][1]);
+                        x[e][2] = __fmaf_rn(v[k][e].z, wk, x[e][2]); x[e][3] = __fmaf_rn(v[k][e].w, wk, x[e][3]);
+                    }
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T* to = reinterpret_cast<T*>(p.y) + row_offset(p, job.t, job.kv_head, job.t.row0 + r);
+            #pragma unroll
+            for (int e = 0; e < PER_LANE; e++) {
+                const int d = (lane + e * 32) * 4;
+                #pragma unroll
+                for (int k = 0; k < 4; k++) x[e][k] *= inv;
+                if (d < p.dim && lane + e * 32 < QUADS) store4(to + d, x[e], p.dim - d, aligned);
+            }
+        }
+        return;
+    }
+    for (int r = row_begin; r < row_end; r++) {
         float top = -INFINITY;
         for (int k = lane; k < job.parts; k += 32) top = fmaxf(top, parts.stats[(long long)slot(k) * N + r].x);
         #pragma unroll
@@ -101,7 +143,8 @@ bool join_partials(const AttentionProblem& p, const PartialResults& parts, int b
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)blocks, N / 4);
+        constexpr int ROWS = N >= 64 ? 32 : 4;
+        cfg.gridDim = dim3((unsigned)blocks, N / ROWS);
         cfg.blockDim = dim3(kJoinThreads);
         cfg.stream = stream;
         cfg.attrs = attr;
@@ -109,7 +152,7 @@ bool join_partials(const AttentionProblem& p, const PartialResults& parts, int b
         AttentionProblem copy = p;
         PartialResults copy_parts = parts;
         void* args[] = {&copy, &copy_parts};
-        ok = check_cuda(cudaLaunchKernelExC(&cfg, (const void*)attention_join<T, N, DIMS>, args), "attention_join");
+        ok = check_cuda(cudaLaunchKernelExC(&cfg, (const void*)attention_join<T, N, DIMS, ROWS>, args), "attention_join");
     }
     return TOPS_CUDA_OK(cudaFreeAsync(parts.o, stream)) && ok;
 }
