@@ -223,6 +223,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     const int from = tiles_at(at.offset), to = tiles_at(at.offset + take);
                     seg.lo = first + from;
                     seg.n = to - from;
+                    if constexpr (MASKED) trim_masked(p, seg.t.seq, seg.t.key_end, seg.lo, seg.n);
                     seg.part = at.offset == 0 && take == at.weight ? -1 : (int)blockIdx.x * 2 + (x == x0 ? 0 : 1);
                     if (seg.part >= 0 && at.offset <= x - x0 && x - at.offset + at.weight > x1)
                         job = JoinJob{seg.t, seg.kv_head, (int)((x - at.offset + at.weight - 1) / share) - (int)blockIdx.x + 1, seg.part};
@@ -427,6 +428,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 all_high = __reduce_min_sync(~0u, high);
                 if (p.window > 0) { low = high - p.window; all_low = __reduce_max_sync(~0u, low); }
             }
+            uint32_t mask_raw[4] = {0u, 0u, 0u, 0u};
+            if constexpr (MASKED) if (n > 0) load_mask(p, t.seq, lo * kChunkKeys + lane, t.key_end, mask_raw);
             float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;          // m in units of the raw score
             for (int i = 0; i < n; i++) {
                 const int j0 = (lo + i) * kChunkKeys;
@@ -436,10 +439,12 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 if constexpr (MASKED) {
                     __syncwarp();                              // the last tile's biases have been read
                     bool some = false;
+                    float four[4];
+                    mask_values(p, mask_raw, j0 + lane, t.key_end, four);
+                    load_mask(p, t.seq, j0 + kChunkKeys + lane, i + 1 < n ? t.key_end : 0, mask_raw);      // the next tile's, on their way during this one
                     #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int j = j0 + e * 32 + lane;
-                        const float b = j < t.key_end ? key_bias(p, t.seq, j) : -INFINITY;
+                        const float b = four[e];
                         warp_bias[warp][e * 32 + lane] = b * per_scale;       // in units of the raw score
                         some = some || b != 0.0f;
                         if (e == quarter) dead = b == -INFINITY;
@@ -495,6 +500,15 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : -m * scale;
+                if (dead) {                                    // a weight of zero times a NaN would still be one
+                    if (!umma::mbar_wait(&full[slot], phase, abort_flag)) ok = false;
+                    uint8_t* key = ring + slot * L::kSlotBytes + row * 128;
+                    #pragma unroll
+                    for (int b = 0; b < DB; b++)
+                        #pragma unroll
+                        for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(key + b * (kChunkKeys * 128) + c * 16) = make_uint4(0, 0, 0, 0);
+                    umma::fence_proxy_async_smem();
+                }
                 #pragma unroll
                 for (int c = 0; c < 128; c += 64) {
                     uint32_t w[32];
@@ -510,15 +524,6 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     umma::tmem_store_32x32(s_at + c / 2, w);
                 }
                 umma::tmem_store_wait();
-                if (dead) {                                    // a weight of zero times a NaN would still be one
-                    if (!umma::mbar_wait(&full[slot], phase, abort_flag)) ok = false;
-                    uint8_t* key = ring + slot * L::kSlotBytes + row * 128;
-                    #pragma unroll
-                    for (int b = 0; b < DB; b++)
-                        #pragma unroll
-                        for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(key + b * (kChunkKeys * 128) + c * 16) = make_uint4(0, 0, 0, 0);
-                    umma::fence_proxy_async_smem();
-                }
                 __syncwarp();
                 umma::fence_before_sync();
                 umma::mbar_arrive(&p_ready[group]);

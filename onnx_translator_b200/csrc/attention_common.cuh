@@ -131,17 +131,57 @@ __device__ __forceinline__ int key_row(const AttentionProblem& p, int seq, int j
 
 // What the mask adds to key j's scores, in units of log2; -Inf excludes the key (the type's lowest value does too, so that
 // a row that is masked throughout is empty rather than a softmax over rounding errors).
+__device__ __forceinline__ float mask_value(uint8_t x) { return x ? 0.0f : -INFINITY; }
+__device__ __forceinline__ float mask_value(float x) { return x <= -3.402823466e+38f ? -INFINITY : x * kLog2E; }
+__device__ __forceinline__ float mask_value(__half h) { const float x = __half2float(h); return x <= -65504.0f ? -INFINITY : x * kLog2E; }
+__device__ __forceinline__ float mask_value(__nv_bfloat16 h) { const float x = __bfloat162float(h); return x <= -3.3895313892515355e+38f ? -INFINITY : x * kLog2E; }
+
 __device__ __forceinline__ float key_bias(const AttentionProblem& p, int seq, int j) {
     const long long at = (long long)seq * p.keys + j;
-    float x;
     switch (p.mask_kind) {
-        case kMaskBytes: return reinterpret_cast<const uint8_t*>(p.mask)[at] ? 0.0f : -INFINITY;
-        case kMaskF32:   x = reinterpret_cast<const float*>(p.mask)[at]; if (x <= -3.402823466e+38f) return -INFINITY; break;
-        case kMaskF16:   x = __half2float(reinterpret_cast<const __half*>(p.mask)[at]); if (x <= -65504.0f) return -INFINITY; break;
-        case kMaskBF16:  x = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.mask)[at]); if (x <= -3.3895313892515355e+38f) return -INFINITY; break;
+        case kMaskBytes: return mask_value(reinterpret_cast<const uint8_t*>(p.mask)[at]);
+        case kMaskF32:   return mask_value(reinterpret_cast<const float*>(p.mask)[at]);
+        case kMaskF16:   return mask_value(reinterpret_cast<const __half*>(p.mask)[at]);
+        case kMaskBF16:  return mask_value(reinterpret_cast<const __nv_bfloat16*>(p.mask)[at]);
         default:         return 0.0f;
     }
-    return x * kLog2E;
+}
+// Keys j, j + 32, j + 64 and j + 96 at once, as they lie in memory (looked at later by mask_values) ...
+__device__ __forceinline__ void load_mask(const AttentionProblem& p, int seq, int j, int key_end, uint32_t (&raw)[4]) {
+    const long long at = (long long)seq * p.keys + j;
+    #pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (j + e * 32 >= key_end) continue;
+        if (p.mask_kind == kMaskBytes) raw[e] = reinterpret_cast<const uint8_t*>(p.mask)[at + e * 32];
+        else if (p.mask_kind == kMaskF32) raw[e] = reinterpret_cast<const uint32_t*>(p.mask)[at + e * 32];
+        else raw[e] = reinterpret_cast<const uint16_t*>(p.mask)[at + e * 32];
+    }
+}
+// ... and what they add; -Inf from key_end on.
+__device__ __forceinline__ void mask_values(const AttentionProblem& p, const uint32_t (&raw)[4], int j, int key_end, float (&b)[4]) {
+    #pragma unroll
+    for (int e = 0; e < 4; e++) {
+        float x;
+        if (p.mask_kind == kMaskBytes) x = mask_value((uint8_t)raw[e]);
+        else if (p.mask_kind == kMaskF32) x = mask_value(__uint_as_float(raw[e]));
+        else if (p.mask_kind == kMaskF16) x = mask_value(__ushort_as_half((unsigned short)raw[e]));
+        else x = mask_value(__ushort_as_bfloat16((unsigned short)raw[e]));
+        b[e] = j + e * 32 < key_end ? x : -INFINITY;
+    }
+}
+
+// Drops the 128-key tiles of [lo, lo + n) at either end whose keys the mask excludes altogether: padding is not copied.  A whole warp, `n` > 0.
+__device__ __forceinline__ void trim_masked(const AttentionProblem& p, int seq, int key_end, int& lo, int& n) {
+    const int lane = threadIdx.x & 31;
+    auto kept = [&](int tile) {
+        uint32_t raw[4] = {0u, 0u, 0u, 0u};
+        float b[4];
+        load_mask(p, seq, tile * 128 + lane, key_end, raw);
+        mask_values(p, raw, tile * 128 + lane, key_end, b);
+        return __any_sync(~0u, b[0] != -INFINITY || b[1] != -INFINITY || b[2] != -INFINITY || b[3] != -INFINITY) != 0;
+    };
+    while (n > 0 && !kept(lo + n - 1)) n--;
+    while (n > 0 && !kept(lo)) { lo++; n--; }
 }
 
 // Element offset of row r of the tile's sequence in q and y (without the dimension).

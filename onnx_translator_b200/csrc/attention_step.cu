@@ -256,6 +256,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 seg.lo = max(first + at.unit, seg.t.key_begin / kStepKeys);
                 const int all = (seg.t.key_end + kStepKeys - 1) / kStepKeys, hi = whole ? all : min(first + at.unit + take, all);
                 seg.n = seg.t.key_end > seg.t.key_begin ? max(hi - seg.lo, 0) : 0;
+                if (p.mask_kind != kMaskNone) trim_masked(p, seg.t.seq, seg.t.key_end, seg.lo, seg.n);
                 seg.part = at.unit == 0 && take == at.w.units ? -1 : (int)blockIdx.x * 2 + (x == x0 ? 0 : 1);
                 if (seg.part >= 0 && x - at.unit >= x0 && x - at.unit + at.w.units > x1)
                     job = JoinJob{seg.t, seg.kv_head, (x - at.unit + at.w.units - 1) / share - (int)blockIdx.x + 1, seg.part};
@@ -676,10 +677,12 @@ template <typename T, int DB, int N, int SLOTS> static bool launch_step(const At
     return ok;
 }
 
+// Sixteen columns for up to sixteen rows of a sequence (on average), else thirty-two; longer sequences take several row tiles.  Ring slots: as many as shared memory
+// holds with one block per SM -- for heads of 64 with two blocks.
 template <typename T> static bool launch_step_size(const AttentionProblem& p) {
     const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
-    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 5>(p) : rows <= 32 ? launch_step<T, 1, 32, 5>(p) : launch_step<T, 1, 64, 7>(p);
-    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 5>(p) : rows <= 32 ? launch_step<T, 2, 32, 5>(p) : launch_step<T, 2, 64, 4>(p);
+    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 5>(p) : launch_step<T, 1, 32, 8>(p);
+    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 5>(p) : launch_step<T, 2, 32, 5>(p);
     return rows <= 16 ? launch_step<T, 4, 16, 3>(p) : launch_step<T, 4, 32, 2>(p);
 }
 

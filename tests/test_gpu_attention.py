@@ -100,6 +100,34 @@ def test_large_scores(dtype, tokens):
     assert_close(run_paged(problem), want, tol)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 200])
+def test_nan_and_infinity_in_real_keys_show(dtype, tokens):
+    """A NaN in a key that a row sees makes that row NaN, wherever in a tile the key stands; rows that do not see its tile stay as they are."""
+    for at in (0, 1, 2, 3, 5, 6, 7, 37, 126, 130):
+        problem = Paged(_rng(dtype, tokens, "nan"), dtype, 4, 2, 64, 16, [(tokens, 300), (tokens, 260)])
+        page, offset = problem.table[0, at // 16], at % 16
+        problem.key_cache[page, offset, 0, 5] = np.nan
+        got = run_paged(problem)
+        want, tol = problem.want()
+        if tokens <= 300 - at:
+            sees = np.arange(tokens) + 300 - tokens >= at
+            assert np.isnan(got[:tokens][sees, :2]).all()
+        assert_close(got[:, 2:], want[:, 2:], tol[:, 2:])
+        assert_close(got[tokens:], want[tokens:], tol[tokens:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-6, 3.0])
+def test_scales(dtype, scale):
+    """No scale, a negative one, a tiny and a large one."""
+    for tokens in (2, 140):
+        problem = Paged(_rng(dtype, tokens, "scale"), dtype, 4, 2, 64, 16, [(tokens, 300)])
+        problem.scale = scale
+        want, tol = problem.want()
+        assert_close(run_paged(problem), want, tol)
+
+
 @pytest.mark.parametrize("tokens", [1, 200])
 def test_ascending_scores(tokens):
     """Every tile has a larger maximum than all before it."""
@@ -225,6 +253,20 @@ def test_cross_masks(dtype, queries, mask_dtype):
     got = _cross(dtype, 4, queries, 290, 4, 2, 64, mask=mask, mask_dtype=mask_dtype)
     assert np.all(got[1] == 0.0)
     _cross(dtype, 4, queries, 290, 2, 2, 128, lengths=[290, 100, 201, 33], mask=mask, mask_dtype=mask_dtype, heads_first=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [1, 150])
+def test_cross_padding_of_whole_tiles(dtype, queries):
+    """Padding in front, behind and in the middle that is longer than a tile of keys; one row without any key."""
+    mask = np.ones((5, 1111), np.uint8)
+    mask[0, 300:] = 0
+    mask[1, :900] = 0
+    mask[2, 130:1000] = 0
+    mask[3] = 0
+    mask[4, :1110] = 0
+    got = _cross(dtype, 5, queries, 1111, 4, 2, 64, mask=mask)
+    assert np.all(got[3] == 0.0)
 
 
 def test_no_keys_at_all_gives_zeros():
