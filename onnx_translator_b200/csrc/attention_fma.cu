@@ -36,9 +36,11 @@ __global__ void __launch_bounds__(kFmaThreads) attention_fma_kernel(const __grid
     const int lo = min(t.key_begin + rank * share, t.key_end), hi = min(lo + share, t.key_end);
 
     const T* q = reinterpret_cast<const T*>(p.q);
-    for (int i = tid; i < R * DP; i += kFmaThreads) {
-        const int r = i / DP, d = i - r * DP;
-        qs[i] = (r < t.rows && d < dim) ? to_float(q[row_offset(p, t, kv_head, t.row0 + r) + d]) : 0.0f;
+    for (int i = tid; i < R * DP / 4; i += kFmaThreads) {
+        const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
+        const T* row = q + (r < t.rows ? row_offset(p, t, kv_head, t.row0 + r) : 0);
+        #pragma unroll
+        for (int e = 0; e < 4; e++) qs[r * DP + d + e] = r < t.rows && d + e < dim ? to_float(row[d + e]) : 0.0f;
     }
     if (tid < R) stats[tid] = make_float2(-INFINITY, 0.0f);
 

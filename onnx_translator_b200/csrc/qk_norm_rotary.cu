@@ -129,16 +129,29 @@ template <typename T> static bool launch_general(const NormRotaryProblem& p) {
     return TOPS_CHECK_LAUNCH("norm_rotary_general");
 }
 
-// Vector form: dim a multiple of 8 up to 256, 16-byte aligned rows.  LPH lanes hold a head, eight neighbouring elements each, and
-// work through HB heads of one token: all HB loads are in flight before the first use, and the token's cosines and sines are
-// read once for the HB heads.  With pairs (i, i + half) the partner elements sit in another lane of the head (a shuffle), with
-// interleaved pairs in the same lane.
-// Eight elements as they lie in memory.
+// Vector form: dim a multiple of 8 up to 256, 16-byte aligned rows.  LPH lanes hold a head, eight elements each, and work through HB heads of one token, whose
+// cosines and sines are read once for them; all HB loads are in flight while position, slot and table row are looked up.  Issue slots bound it next to HBM:
+// arithmetic is two floats to an instruction, and 64 registers a thread keep 32 warps on an SM (112 us with 80 of them, 94 us with 64: 4.4 TB/s).  (Fetching the next item ahead was measured and is not done: its registers cost more warps than it hid, 166 against 122 us
+// for 16384 tokens of 32 + 2 * 8 heads of 128.)
+// Three layouts of a head over the lanes: eight neighbours with interleaved pairs; four and four elements half a head apart where
+// the whole head is turned in pairs (i, i + half), so that a lane holds both elements of its pairs; eight neighbours and a shuffle to the partner's lane
+// where only part of the head is turned.
+enum RotaryLayout { kLayoutInterleaved = 0, kLayoutPaired = 1, kLayoutShuffled = 2 };
+
+// Eight elements as they lie in memory: at d and d + 4, or (paired) four at each of two places.
 template <typename T> struct Raw8 { uint4 w[sizeof(T) / 2]; };
-template <typename T> __device__ __forceinline__ Raw8<T> load_raw8(const T* from) {
+template <typename T, bool PAIRED> __device__ __forceinline__ Raw8<T> load_raw8(const T* first, int apart) {
     Raw8<T> r;
-    #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = reinterpret_cast<const uint4*>(from)[i];
+    if constexpr (PAIRED && sizeof(T) == 2) {
+        const uint2 a = *reinterpret_cast<const uint2*>(first), b = *reinterpret_cast<const uint2*>(first + apart);
+        r.w[0] = make_uint4(a.x, a.y, b.x, b.y);
+    } else if constexpr (PAIRED) {
+        r.w[0] = *reinterpret_cast<const uint4*>(first);
+        r.w[1] = *reinterpret_cast<const uint4*>(first + apart);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = reinterpret_cast<const uint4*>(first)[i];
+    }
     return r;
 }
 template <typename T> __device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
@@ -146,29 +159,43 @@ template <typename T> __device__ __forceinline__ void widen8(const Raw8<T>& r, f
     #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = to_float(t[i]);
 }
-template <typename T> __device__ __forceinline__ void load8(const T* from, float (&x)[8]) { widen8(load_raw8(from), x); }
-template <typename T> __device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
+template <typename T, bool PAIRED> __device__ __forceinline__ void load8(const T* first, int apart, float (&x)[8]) { widen8(load_raw8<T, PAIRED>(first, apart), x); }
+template <typename T, bool PAIRED> __device__ __forceinline__ void store8(T* to, int apart, const float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
         reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        *reinterpret_cast<float4*>(to + (PAIRED ? apart : 4)) = make_float4(x[4], x[5], x[6], x[7]);
+    } else if constexpr (PAIRED) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+        *reinterpret_cast<uint2*>(to + apart) = make_uint2(pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
     } else {
         *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
     }
 }
 
+// r = a * b (+ c) for two floats in one instruction.
+__device__ __forceinline__ void mul_pair(float& r0, float& r1, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma_pair(float& r0, float& r1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
 constexpr int kNormThreads = 128;
 
-template <typename T, int LPH, int HB, bool INTERLEAVED>
-__global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_constant__ NormRotaryProblem p, const uint32_t items) {
+template <typename T, int LPH, int HB, int LAYOUT>
+__global__ void __launch_bounds__(kNormThreads, sizeof(T) == 2 ? 8 : 6) norm_rotary_vector(const __grid_constant__ NormRotaryProblem p, const uint32_t items) {
     constexpr int PER_WARP = 32 / LPH;
+    constexpr bool PAIRED = LAYOUT == kLayoutPaired;
     const int lane = threadIdx.x & 31, in_head = lane % LPH, group = lane / LPH;
     const uint32_t warp = blockIdx.x * (kNormThreads / 32) + (threadIdx.x >> 5), warps = gridDim.x * (kNormThreads / 32);
-    const int d = in_head * 8;
-    const bool mine = d < p.dim;
-    const int half = p.half;
-    // the lane that holds the other halves of this lane's pairs
-    const bool second = !INTERLEAVED && d >= half;
-    const int partner = (lane - in_head) + (d < 2 * half ? (second ? d - half : d + half) / 8 : in_head);
+    const int half = p.half, d = in_head * (PAIRED ? 4 : 8);
+    const bool mine = in_head * 8 < p.dim;
+    // shuffled: the lane that holds the other elements of this lane's pairs
+    const bool second = LAYOUT == kLayoutShuffled && d >= half;
+    const int partner = LAYOUT == kLayoutShuffled ? (lane - in_head) + (d < 2 * half ? (second ? d - half : d + half) / 8 : in_head) : lane;
+
     for (uint32_t base = warp * PER_WARP; base < items; base += warps * PER_WARP) {
         const uint32_t item = base + group;
         const bool there = item < items;
@@ -176,24 +203,23 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_
         int block = (int)((there ? item : 0u) - token * p.block_div.d), which = 0;
         if (block >= p.blocks[0]) { block -= p.blocks[0]; which = 1; if (block >= p.blocks[1]) { block -= p.blocks[1]; which = 2; } }
         const HeadsView& h = p.part[which];
-        const int head0 = block * HB;
-        const int batch = (int)p.seq_div.div(token), in_row = (int)token - batch * p.seq;
+        const int head0 = block * HB, batch = (int)p.seq_div.div(token), in_row = (int)token - batch * p.seq;
         const T* in = reinterpret_cast<const T*>(h.in) + batch * h.in_batch + in_row * h.in_token + head0 * h.in_head + d;
-        Raw8<T> raw[HB];                                     // on their way while position, slot and table row are looked up
+        Raw8<T> raw[HB];
         #pragma unroll
-        for (int i = 0; i < HB; i++) if (there && mine && head0 + i < h.heads) raw[i] = load_raw8(in + i * h.in_head);
+        for (int i = 0; i < HB; i++) if (there && mine && head0 + i < h.heads) raw[i] = load_raw8<T, PAIRED>(in + i * h.in_head, half);
         const bool normed = h.weight && mine;
         float w[8];
         if (normed) {
-            if (h.weight_f32) load8(reinterpret_cast<const float*>(h.weight) + d, w);
-            else load8(reinterpret_cast<const T*>(h.weight) + d, w);
+            if (h.weight_f32) load8<float, PAIRED>(reinterpret_cast<const float*>(h.weight) + d, half, w);
+            else load8<T, PAIRED>(reinterpret_cast<const T*>(h.weight) + d, half, w);
         }
         const TokenPlace at = place_token(p, (int)token, p.positions != nullptr, h.cache != nullptr);
-        constexpr int N = INTERLEAVED ? 4 : 8;
+        constexpr int N = LAYOUT == kLayoutShuffled ? 8 : 4;
         float c[N], s[N];
-        const bool turned = h.rotate && at.table_row >= 0 && d < 2 * half;
+        const bool turned = h.rotate && at.table_row >= 0 && (PAIRED ? mine : d < 2 * half);
         if (turned) {
-            const long long row = (long long)at.table_row * half + (INTERLEAVED ? d / 2 : (second ? d - half : d));
+            const long long row = (long long)at.table_row * half + (LAYOUT == kLayoutInterleaved ? d / 2 : (second ? d - half : d));
             #pragma unroll
             for (int e = 0; e < N; e += 4) {
                 const float4 cv = *reinterpret_cast<const float4*>(p.cos_table + row + e), sv = *reinterpret_cast<const float4*>(p.sin_table + row + e);
@@ -203,6 +229,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_
         }
         T* out = h.out ? reinterpret_cast<T*>(h.out) + batch * h.out_batch + in_row * h.out_token + head0 * h.out_head + d : nullptr;
         T* cache = h.cache && at.slot >= 0 && !at.bad_position ? reinterpret_cast<T*>(h.cache) + (at.slot * p.cache_heads + head0) * p.dim + d : nullptr;
+        const bool any_normed = __any_sync(~0u, normed);     // the groups of a warp may be in different parts: all of them reduce, or none
         #pragma unroll
         for (int i = 0; i < HB; i++) {
             const bool here = there && mine && head0 + i < h.heads;
@@ -212,36 +239,44 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_
                 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e] = 0.0f;
             }
-            float sum = 0.0f;                                // the groups of a warp may be in different parts: all of them reduce
-            #pragma unroll
-            for (int e = 0; e < 8; e++) sum = __fmaf_rn(x[e], x[e], sum);
-            #pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            const float factor = rsqrtf(__fmaf_rn(sum, p.inv_dim, p.epsilon));
-            if (normed)
+            if (any_normed) {
+                float sum0 = 0.0f, sum1 = 0.0f;
                 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = x[e] * factor * w[e];
-            if constexpr (INTERLEAVED) {
-                if (turned)
+                for (int e = 0; e < 8; e += 2) fma_pair(sum0, sum1, x[e], x[e + 1], x[e], x[e + 1], sum0, sum1);
+                float sum = sum0 + sum1;
+                #pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+                const float factor = rsqrtf(__fmaf_rn(sum, p.inv_dim, p.epsilon));
+                if (normed)
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float a = x[2 * e], b = x[2 * e + 1];
-                        x[2 * e] = __fmaf_rn(a, c[e], -(b * s[e]));
-                        x[2 * e + 1] = __fmaf_rn(a, s[e], b * c[e]);
+                    for (int e = 0; e < 8; e += 2) {
+                        mul_pair(x[e], x[e + 1], x[e], x[e + 1], factor, factor);
+                        mul_pair(x[e], x[e + 1], x[e], x[e + 1], w[e], w[e + 1]);
                     }
-            } else if (half > 0) {
+            }
+            if constexpr (LAYOUT == kLayoutShuffled) {
                 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float other = __shfl_sync(~0u, x[e], partner);
                     if (turned) x[e] = second ? __fmaf_rn(other, s[e], x[e] * c[e]) : __fmaf_rn(x[e], c[e], -(other * s[e]));
+                }
+            } else if (turned) {
+                #pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const int a0 = PAIRED ? e : 2 * e, a1 = PAIRED ? e + 1 : 2 * e + 2, b0 = PAIRED ? e + 4 : 2 * e + 1, b1 = PAIRED ? e + 5 : 2 * e + 3;
+                    float t0, t1, u0, u1;
+                    mul_pair(t0, t1, x[b0], x[b1], -s[e], -s[e + 1]);
+                    mul_pair(u0, u1, x[b0], x[b1], c[e], c[e + 1]);
+                    fma_pair(x[b0], x[b1], x[a0], x[a1], s[e], s[e + 1], u0, u1);
+                    fma_pair(x[a0], x[a1], x[a0], x[a1], c[e], c[e + 1], t0, t1);
                 }
             }
             if (here) {
                 if (at.bad_position)
                     #pragma unroll
                     for (int e = 0; e < 8; e++) x[e] = 0.0f;
-                if (out) store8(out + i * h.out_head, x);
-                if (cache) store8(cache + (long long)i * p.dim, x);
+                if (out) store8<T, PAIRED>(out + i * h.out_head, half, x);
+                if (cache) store8<T, PAIRED>(cache + (long long)i * p.dim, half, x);
             }
         }
     }
@@ -249,7 +284,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_rotary_vector(const __grid_
 
 // Whether every row that the vector form reads or writes starts on a 16-byte boundary, and pairs are met lane by lane.
 static bool vector_form(const NormRotaryProblem& p) {
-    if (p.dim % 8 != 0 || p.dim > 256 || p.half % 4 != 0 || (!p.interleaved && p.half % 8 != 0)) return false;
+    if (p.dim % 8 != 0 || p.dim > 256 || p.half % 4 != 0 || (!p.interleaved && 2 * p.half != p.dim && p.half % 8 != 0)) return false;
     uintptr_t bits = reinterpret_cast<uintptr_t>(p.cos_table) | reinterpret_cast<uintptr_t>(p.sin_table);
     for (const HeadsView& h : p.part)
         for (const void* a : {h.in, (const void*)h.out, (const void*)h.cache, h.weight}) bits |= reinterpret_cast<uintptr_t>(a);
@@ -264,15 +299,17 @@ template <typename T, int LPH, int HB> static bool launch_vector(NormRotaryProbl
     p.block_div.set((uint32_t)blocks);
     const uint32_t items = (uint32_t)p.tokens * (uint32_t)blocks;
     const int grid = grid_for(items, kNormThreads / LPH, st->sm_count, 16);
-    if (p.interleaved) norm_rotary_vector<T, LPH, HB, true><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
-    else norm_rotary_vector<T, LPH, HB, false><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
+    if (p.interleaved || p.half == 0) norm_rotary_vector<T, LPH, HB, kLayoutInterleaved><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
+    else if (2 * p.half == p.dim) norm_rotary_vector<T, LPH, HB, kLayoutPaired><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
+    else norm_rotary_vector<T, LPH, HB, kLayoutShuffled><<<grid, kNormThreads, 0, current_stream()>>>(p, items);
     return TOPS_CHECK_LAUNCH("norm_rotary_vector");
 }
 
 template <typename T, int LPH> static bool launch_vector_heads(const NormRotaryProblem& p) {
-    // four heads per group share a token's table row; with few heads in all, one each spreads them over more SMs
+    // four heads per group share a token's table row (measured 94 us, two 121, eight 149 for 16384 tokens of 48 heads of 128); with too few heads to give every SM 512
+    // threads that way, one each spreads them further
     const long long heads = (long long)p.tokens * (p.part[0].heads + p.part[1].heads + p.part[2].heads);
-    return heads * LPH >= (long long)kNumSMs * 2048 * 4 ? launch_vector<T, LPH, 4>(p) : launch_vector<T, LPH, 1>(p);
+    return heads * LPH >= (long long)kNumSMs * 512 * 4 ? launch_vector<T, LPH, 4>(p) : launch_vector<T, LPH, 1>(p);
 }
 
 template <typename T> static bool launch_any(const NormRotaryProblem& p) {
