@@ -177,6 +177,6 @@ def synchronize() -> None:
     capi.check(lib)
 
 
-from .graph import Graph, qdq_resnet50, small_cnn  # noqa: E402  (the graph runner builds on the classes above)
+from .graph import Graph, cached_decoder_layer, qdq_resnet50, small_cnn  # noqa: E402  (the graph runner builds on the classes above)
 from .plan import GraphPlan  # noqa: E402
 from .attention_ops import CrossAttention, PagedAttention, QKNormRotary  # noqa: E402

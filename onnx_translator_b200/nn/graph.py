@@ -471,3 +471,57 @@ def qdq_resnet50(batch: int = 256, seed: int = 0, image: int = 224, stages: Sequ
     graph = Graph(b.nodes, "x", ["prob"], "qdq_resnet50", b.init)
     graph.macs_per_image = b.macs_per_image + classes * c_in
     return graph, _tensor(x, f32)
+
+
+def cached_decoder_layer(batch: int, heads: int = 8, kv_heads: int = 2, dim: int = 64, pages: int = 64, page_size: int = 16, reach: int = 4096,
+                         seed: int = 0, dtype: str = "bfloat16"):
+    """The attention half of an encoder-decoder layer for one new token per sequence, over a paged cache that the graph owns:
+    projection -> norms, rotation and append -> paged attention -> projection -> Add -> attention to the encoder's states ->
+    projection -> Add, with seeded weights.
+
+    Graph inputs: x [batch, heads * dim]; positions and slots int32 [batch]; page_table int32 [batch, width], query_start int32
+    [batch + 1], kv_length int32 [batch] (the new token included); enc_k, enc_v [batch, keys, kv_heads, dim]; enc_length int32 [batch].
+    Outputs: "y" and the edges "qkv", "q", "seen", "cross_q", "crossed" in front of and behind the attention nodes.  The caches are the
+    initializers "key_cache" and "value_cache" [pages, page_size, kv_heads, dim], written in place by every run."""
+    from . import Operators as ops
+    from .attention_ops import CrossAttention, PagedAttention, QKNormRotary
+    from . import Tensor
+    rng = np.random.default_rng(seed)
+    width = heads * dim
+
+    def normal(*shape, spread):
+        codes = rng.normal(0, spread, shape).astype(np.float32)
+        if dtype == "bfloat16":                       # round to the nearest bfloat16
+            u = codes.view(np.uint32)
+            codes = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+        elif dtype == "float16":
+            codes = codes.astype(np.float16)
+        return _tensor(codes, dtype)
+
+    angle = np.arange(reach)[:, None] * 10000.0 ** (-np.arange(0, dim, 2) / dim)
+    cache_shape = (pages, page_size, kv_heads, dim)
+    init = {
+        "w_qkv": normal(width, (heads + 2 * kv_heads) * dim, spread=width ** -0.5), "w_o": normal(width, width, spread=width ** -0.5),
+        "w_cross": normal(width, width, spread=width ** -0.5), "w_cross_o": normal(width, width, spread=width ** -0.5),
+        "q_norm": normal(dim, spread=1.0), "k_norm": normal(dim, spread=1.0),
+        "cos": _tensor(np.cos(angle).astype(np.float32), "float32"), "sin": _tensor(np.sin(angle).astype(np.float32), "float32"),
+        "key_cache": Tensor(*cache_shape, dtype=dtype), "value_cache": Tensor(*cache_shape, dtype=dtype),
+    }
+    nodes = [
+        ops.MatMul(["x", "w_qkv"], ["qkv2"], dtype=dtype),
+        ops.Reshape(["qkv2"], ["qkv"], shape=[batch, heads + 2 * kv_heads, dim], dtype=dtype),
+        QKNormRotary(["qkv", "", "", "q_norm", "k_norm", "cos", "sin", "positions", "key_cache", "value_cache", "slots"], ["q"],
+                     packed_kv_heads=kv_heads, dtype=dtype),
+        PagedAttention(["q", "key_cache", "value_cache", "page_table", "query_start", "kv_length"], ["seen"], dtype=dtype),
+        ops.Reshape(["seen"], ["seen2"], shape=[batch, width], dtype=dtype),
+        ops.MatMul(["seen2", "w_o"], ["o"], dtype=dtype),
+        ops.ADD(["x", "o"], ["h"], dtype=dtype),
+        ops.MatMul(["h", "w_cross"], ["cross_q2"], dtype=dtype),
+        ops.Reshape(["cross_q2"], ["cross_q"], shape=[batch, 1, heads, dim], dtype=dtype),
+        CrossAttention(["cross_q", "enc_k", "enc_v", "enc_length"], ["crossed"], dtype=dtype),
+        ops.Reshape(["crossed"], ["crossed2"], shape=[batch, width], dtype=dtype),
+        ops.MatMul(["crossed2", "w_cross_o"], ["co"], dtype=dtype),
+        ops.ADD(["h", "co"], ["y"], dtype=dtype),
+    ]
+    inputs = ["x", "positions", "slots", "page_table", "query_start", "kv_length", "enc_k", "enc_v", "enc_length"]
+    return Graph(nodes, inputs, ["y", "qkv", "q", "seen", "cross_q", "crossed"], "cached_decoder_layer", init)
