@@ -157,46 +157,42 @@ __device__ __forceinline__ bool any_of_softmax(int group, bool x) {
 }
 __device__ __forceinline__ void softmax_sync(int group) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory"); }
 
-template <int N> __device__ __forceinline__ void tmem_load_columns(uint32_t at, float (&x)[N]) {
-    if constexpr (N == 16) {
-        uint32_t r[16];
-        umma::tmem_load_32x16(at, r);
-        umma::tmem_load_wait();
-        #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = __uint_as_float(r[i]);
-    } else {
-        #pragma unroll
-        for (int c = 0; c < N; c += 32) {
-            uint32_t r[32];
-            umma::tmem_load_32x32(at + c, r);
-            umma::tmem_load_wait();
-            #pragma unroll
-            for (int i = 0; i < 32; i++) x[c + i] = __uint_as_float(r[i]);
-        }
-    }
+template <int W> __device__ __forceinline__ void tmem_load_some(uint32_t at, uint32_t (&r)[W]) {
+    if constexpr (W == 4) umma::tmem_load_32x4(at, r);
+    else if constexpr (W == 8) umma::tmem_load_32x8(at, r);
+    else if constexpr (W == 16) umma::tmem_load_32x16(at, r);
+    else umma::tmem_load_32x32(at, r);
 }
-// The N columns of one accumulator times the rows' factors.
-template <int N> __device__ __forceinline__ void tmem_scale_columns(uint32_t at, const float* factor) {
-    constexpr int W = N == 16 ? 16 : 32;
+// The first R columns of one accumulator.
+template <int R> __device__ __forceinline__ void tmem_load_columns(uint32_t at, float (&x)[R]) {
+    uint32_t r[R];
+    tmem_load_some<R>(at, r);
+    umma::tmem_load_wait();
     #pragma unroll
-    for (int c = 0; c < N; c += W) {
-        uint32_t r[W];
-        if constexpr (W == 16) umma::tmem_load_32x16(at + c, r); else umma::tmem_load_32x32(at + c, r);
-        umma::tmem_load_wait();
-        #pragma unroll
-        for (int i = 0; i < W; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor[c + i]);
-        if constexpr (W == 16) umma::tmem_store_32x16(at + c, r); else umma::tmem_store_32x32(at + c, r);
-    }
+    for (int i = 0; i < R; i++) x[i] = __uint_as_float(r[i]);
+}
+// The same times the rows' factors, in place.
+template <int R> __device__ __forceinline__ void tmem_scale_columns(uint32_t at, const float* factor) {
+    uint32_t r[R];
+    tmem_load_some<R>(at, r);
+    umma::tmem_load_wait();
+    #pragma unroll
+    for (int i = 0; i < R; i++) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor[i]);
+    if constexpr (R == 4) umma::tmem_store_32x4(at, r);
+    else if constexpr (R == 8) umma::tmem_store_32x8(at, r);
+    else if constexpr (R == 16) umma::tmem_store_32x16(at, r);
+    else umma::tmem_store_32x32(at, r);
     umma::tmem_store_wait();
 }
 
 constexpr float kNoMaximum = -3.402823466e+38f;               // finite, so that score - m is never Inf - Inf
 constexpr float kMaximumSlack = 8.0f;
 
-template <typename T, int DB, int N, int SLOTS>
+template <typename T, int DB, int R, int SLOTS>
 __global__ void __launch_bounds__(kStepThreads)
 attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       const __grid_constant__ AttentionProblem p, const int box_rows, const PartialResults parts) {
+    constexpr int N = R > 16 ? 32 : 16;                       // columns of the instructions; rows beyond R are zero queries whose results nobody reads
     using L = StepLayout<DB, N, SLOTS>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[SLOTS], s_full[4], p_ready[2], pv_done[4], seg_full[2], seg_empty[2], o_full[2], turn[2], drained;
@@ -204,8 +200,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     __shared__ int abort_word, drain_word;
     __shared__ __align__(16) unsigned char segment_memory[2 * sizeof(Segment)];
     Segment* segments = reinterpret_cast<Segment*>(segment_memory);
-    __shared__ __align__(16) float group_floats[2][7 * N];    // per softmax group: warp_top[4], fade, top_of, sums
-    __shared__ int group_high[2][N];
+    __shared__ __align__(16) float group_floats[2][7 * R];    // per softmax group: warp_top[4], fade, top_of, sums
+    __shared__ int group_high[2][R];
     uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* q_tiles = ring + SLOTS * L::kSlotBytes;
     uint8_t* p_tile = q_tiles + 2 * L::kQBytes;
@@ -220,7 +216,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         abort_word = drain_word = 0;
         umma::mbar_fence_init();
     }
-    if (threadIdx.x < 2 * N) group_floats[threadIdx.x / N][4 * N + threadIdx.x % N] = 1.0f;      // fade of the columns that no row uses
+    if (threadIdx.x < 2 * R) group_floats[threadIdx.x / R][4 * R + threadIdx.x % R] = 1.0f;      // fade of the columns that no row uses
     if (warp == 4 && lane == 0) { umma::tma_prefetch_desc(&k_map); umma::tma_prefetch_desc(&v_map); }
     // Scheduled while the previous kernel of the stream drains; nothing so far has touched global or tensor memory.  The join in turn may be scheduled early: it
     // waits for this grid before it reads.
@@ -236,7 +232,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     if (warp == 6) {
         // ---- items: what this block works on, and its queries ---------------------------------------------------------------
         const bool whole = parts.o == nullptr;                 // the unit is the item: nothing is split, nothing joined
-        const int total = total_units<N>(p, whole);
+        const int total = total_units<R>(p, whole);
         const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
         const int x0 = min((int)blockIdx.x * share, total), x1 = min(x0 + share, total);
         int x = x0, s = 0;
@@ -248,8 +244,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             seg.n = -1;
             int page = 0;
             if (x < x1) {
-                at = place_unit<N>(p, x, whole);
-                seg.t = row_tile_of<N>(p, at);
+                at = place_unit<R>(p, x, whole);
+                seg.t = row_tile_of<R>(p, at);
                 seg.kv_head = at.kv_head;
                 const int take = min(at.w.units - at.unit, x1 - x), first = first_tile_of(p, at);
                 // the units counted for the sequence may reach past the keys of this row tile
@@ -441,8 +437,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         // ---- softmax: a thread per key -------------------------------------------------------------------------------------
         const int group = warp >> 3, quarter = warp & 3, key = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)quarter << 21;        // this warp's quarter of tensor memory
-        float (*warp_top)[N] = reinterpret_cast<float (*)[N]>(group_floats[group]);
-        float *fade = group_floats[group] + 4 * N, *top_of = fade + N, *sums = top_of + N;
+        float (*warp_top)[R] = reinterpret_cast<float (*)[R]>(group_floats[group]);
+        float *fade = group_floats[group] + 4 * R, *top_of = fade + R, *sums = top_of + R;
         int* high = group_high[group];
         const bool masked = p.mask_kind != kMaskNone;
         uint32_t slot = 0, phase = 0, o_phase = 0;             // o_phase counts this group's items that had a key
@@ -468,7 +464,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 continue;
             }
             const int rows = seg.t.rows, key_end = seg.t.key_end, lo = seg.lo;
-            if (key < N) {
+            if (key < R) {
                 high[key] = p.page_table ? seg.t.first_position + (int)p.group_div.div((uint32_t)(seg.t.row0 + min(key, rows - 1))) + 1 : key_end;
                 top_of[key] = kNoMaximum;
             }
@@ -476,11 +472,11 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             int all_high = key_end, all_low = 0;
             if (p.page_table) {
                 all_high = high[0];
-                if (p.window > 0) all_low = high[N - 1] - p.window;
+                if (p.window > 0) all_low = high[R - 1] - p.window;
             }
-            float l[N];
+            float l[R];
             #pragma unroll
-            for (int r = 0; r < N; r++) l[r] = 0.0f;
+            for (int r = 0; r < R; r++) l[r] = 0.0f;
             for (int it = 0; it < n; it++, i++) {
                 const int j0 = (lo + it) * kStepKeys, j = j0 + key;
                 if (++slot == SLOTS) { slot = 0; phase ^= 1u; }    // the slot of this tile's values
@@ -493,12 +489,12 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 }
                 if (!umma::mbar_wait(&s_full[i & 3], (uint32_t)(i >> 2) & 1u, abort_flag)) ok = false;
                 umma::fence_after_sync();
-                float z[N];
+                float z[R];
                 __syncwarp();
-                tmem_load_columns<N>(tmem + lanes + (i & 1) * N, z);
+                tmem_load_columns<R>(tmem + lanes + (i & 1) * N, z);
                 float over = -INFINITY;
                 #pragma unroll
-                for (int c = 0; c < N; c += 4)
+                for (int c = 0; c < R; c += 4)
                     if (c < rows) {
                         const float4 m = *reinterpret_cast<const float4*>(top_of + c);
                         const float mr[4] = {m.x, m.y, m.z, m.w};
@@ -516,7 +512,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 if (any_of_softmax(group, over > kMaximumSlack || !ok)) {
                     if (any_of_softmax(group, !ok)) { ok = false; break; }        // a wait has run out: all leave
                     #pragma unroll
-                    for (int c = 0; c < N; c += 4)
+                    for (int c = 0; c < R; c += 4)
                         if (c < rows)
                             #pragma unroll
                             for (int r = c; r < c + 4; r++) {
@@ -526,7 +522,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                                 if (lane == 0) warp_top[quarter][r] = top;
                             }
                     softmax_sync(group);
-                    if (key < N && (key & ~3) < rows) {
+                    if (key < R && (key & ~3) < rows) {
                         const float old = top_of[key];
                         const float top = fmaxf(old, fmaxf(fmaxf(warp_top[0][key], warp_top[1][key]), fmaxf(warp_top[2][key], warp_top[3][key])));
                         fade[key] = exp2_approx(old - top);
@@ -534,7 +530,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                     }
                     softmax_sync(group);
                     #pragma unroll
-                    for (int c = 0; c < N; c += 4)
+                    for (int c = 0; c < R; c += 4)
                         if (c < rows) {
                             const float4 f = *reinterpret_cast<const float4*>(fade + c);
                             l[c] *= f.x; l[c + 1] *= f.y; l[c + 2] *= f.z; l[c + 3] *= f.w;
@@ -544,13 +540,13 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                         umma::fence_after_sync();
                         __syncwarp();
                         #pragma unroll
-                        for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<N>(my_o + a * N, fade);
+                        for (int a = 0; a < L::kOAccs; a++) tmem_scale_columns<R>(my_o + a * N, fade);
                     }
                 }
                 if (i > 1 && !umma::mbar_wait(&pv_done[(i - 2) & 3], (uint32_t)((i - 2) >> 2) & 1u, abort_flag)) ok = false;    // the weights of tile i - 2 are read
                 uint8_t* to = p_tile + (i & 1) * L::kPBytes + (key >> 6) * (N * 128) + (key & 7) * 2;
                 #pragma unroll
-                for (int c = 0; c < N; c += 4)
+                for (int c = 0; c < R; c += 4)
                     if (c < rows) {
                         const float4 m = *reinterpret_cast<const float4*>(top_of + c);
                         const float mr[4] = {m.x, m.y, m.z, m.w};
@@ -584,12 +580,12 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 o_phase ^= 1u;
             }
             __syncwarp();
-            float x[L::kOAccs][N];
+            float x[L::kOAccs][R];
             #pragma unroll
-            for (int a = 0; a < L::kOAccs; a++) tmem_load_columns<N>(my_o + a * N, x[a]);
+            for (int a = 0; a < L::kOAccs; a++) tmem_load_columns<R>(my_o + a * N, x[a]);
             // sums of weights over the keys
             #pragma unroll
-            for (int c = 0; c < N; c += 4)
+            for (int c = 0; c < R; c += 4)
                 if (c < rows)
                     #pragma unroll
                     for (int r = c; r < c + 4; r++) {
@@ -602,7 +598,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             if (key < rows) {
                 const float sum = (warp_top[0][key] + warp_top[1][key]) + (warp_top[2][key] + warp_top[3][key]);
                 sums[key] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (seg.part >= 0) parts.stats[(long long)seg.part * N + key] = make_float2(sum == 0.0f ? -INFINITY : top_of[key], sum);
+                if (seg.part >= 0) parts.stats[(long long)seg.part * R + key] = make_float2(sum == 0.0f ? -INFINITY : top_of[key], sum);
             }
             softmax_sync(group);
             if (seg.part >= 0) {
@@ -611,7 +607,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                     const int d = a * 128 + key;
                     if (d < L::kDims)
                         #pragma unroll
-                        for (int r = 0; r < N; r++) if (r < rows) parts.o[((long long)seg.part * N + r) * L::kDims + d] = x[a][r];
+                        for (int r = 0; r < R; r++) if (r < rows) parts.o[((long long)seg.part * R + r) * L::kDims + d] = x[a][r];
                 }
             } else {
                 #pragma unroll
@@ -619,7 +615,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                     const int d = a * 128 + key;
                     if (d < p.dim)
                         #pragma unroll
-                        for (int r = 0; r < N; r++)
+                        for (int r = 0; r < R; r++)
                             if (r < rows) reinterpret_cast<T*>(p.y)[row_offset(p, seg.t, seg.kv_head, seg.t.row0 + r) + d] = from_float<T>(sums[r] == 0.0f ? 0.0f : x[a][r] * sums[r]);
                 }
             }
@@ -637,7 +633,8 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     }
 }
 
-template <typename T, int DB, int N, int SLOTS> static bool launch_step(const AttentionProblem& p) {
+template <typename T, int DB, int R, int SLOTS> static bool launch_step(const AttentionProblem& p) {
+    constexpr int N = R > 16 ? 32 : 16;
     using L = StepLayout<DB, N, SLOTS>;
     DeviceState* st = acquire_device();
     if (!st) return false;
@@ -647,18 +644,18 @@ template <typename T, int DB, int N, int SLOTS> static bool launch_step(const At
         set_error(TOPS_ERR_CUDA, "attention_step: the tensor map was refused");
         return false;
     }
-    const void* kernel = (const void*)attention_step_kernel<T, DB, N, SLOTS>;
+    const void* kernel = (const void*)attention_step_kernel<T, DB, R, SLOTS>;
     if (!ensure_dynamic_smem(kernel, L::kSmem)) return false;
     // One block per SM (two of the small ones: with heads of 64 a tile is half as long to copy but not to work on), but none that cannot get a tile.  Where an item cannot have more than four tiles (512 keys), a block takes it whole: the join costs as much as
     // three tiles in a row.
-    const long long units = (p.keys + kStepKeys - 1) / kStepKeys, items = attention_tiles(p, N) * p.kv_heads;
+    const long long units = (p.keys + kStepKeys - 1) / kStepKeys, items = attention_tiles(p, R) * p.kv_heads;
     const bool whole = units <= 4;
     const long long most = whole ? items : items * units;
     const long long room = (long long)st->sm_count * (DB == 1 && N == 16 ? 2 : 1);
     const int blocks = (int)(most < room ? most : room);
     cudaStream_t stream = current_stream();
     PartialResults parts;
-    if (!whole && !allocate_partials(parts, blocks, N, L::kDims, stream)) return false;
+    if (!whole && !allocate_partials(parts, blocks, R, L::kDims, stream)) return false;
     AttentionProblem copy = p;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -672,23 +669,29 @@ template <typename T, int DB, int N, int SLOTS> static bool launch_step(const At
     cfg.numAttrs = 1;
     void* args[] = {&k_map, &v_map, &copy, &box_rows, &parts};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_step");
-    if (!whole) ok = join_partials<T, N, L::kDims>(copy, parts, blocks, stream, ok);
+    if (!whole) ok = join_partials<T, R, L::kDims>(copy, parts, blocks, stream, ok);
     if (ok) count_tensor_core_launch();
     return ok;
 }
 
-// Sixteen columns for up to sixteen rows of a sequence (on average), else thirty-two; longer sequences take several row tiles.  Ring slots: as many as shared memory
-// holds with one block per SM -- for heads of 64 with two blocks.
-template <typename T> static bool launch_step_size(const AttentionProblem& p) {
+// Room for 4, 8, 16 or 32 rows, by the rows of a sequence on average (longer sequences take several row tiles): the softmax and its code shrink with it.  Ring
+// slots: as many as shared memory holds with one block per SM -- for heads of 64 with two blocks.
+template <typename T, int DB, int SLOTS, int SLOTS32> static bool launch_step_rows(const AttentionProblem& p) {
     const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
-    if (p.dim <= 64) return rows <= 16 ? launch_step<T, 1, 16, 5>(p) : launch_step<T, 1, 32, 8>(p);
-    if (p.dim <= 128) return rows <= 16 ? launch_step<T, 2, 16, 5>(p) : launch_step<T, 2, 32, 5>(p);
-    return rows <= 16 ? launch_step<T, 4, 16, 3>(p) : launch_step<T, 4, 32, 2>(p);
+    if (rows <= 4) return launch_step<T, DB, 4, SLOTS>(p);
+    if (rows <= 8) return launch_step<T, DB, 8, SLOTS>(p);
+    return rows <= 16 ? launch_step<T, DB, 16, SLOTS>(p) : launch_step<T, DB, 32, SLOTS32>(p);
+}
+
+template <typename T> static bool launch_step_size(const AttentionProblem& p) {
+    if (p.dim <= 64) return launch_step_rows<T, 1, 5, 8>(p);
+    if (p.dim <= 128) return launch_step_rows<T, 2, 5, 5>(p);
+    return launch_step_rows<T, 4, 3, 2>(p);
 }
 
 // The units of the whole problem are counted in 32 bits.
 bool attention_step_fits(const AttentionProblem& p) {
-    return attention_tiles(p, 16) * p.kv_heads * ((p.keys + kStepKeys - 1) / kStepKeys + 1) < 0x40000000ll;
+    return attention_tiles(p, 4) * p.kv_heads * ((p.keys + kStepKeys - 1) / kStepKeys + 1) < 0x40000000ll;
 }
 
 bool attention_step(const AttentionProblem& p) {
