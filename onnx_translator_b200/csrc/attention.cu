@@ -124,8 +124,8 @@ TOPS_API int tops_paged_attention_forward(const PagedAttentionCall* call) {
     p.table_width = c.page_table->shape[1];
     const char* limit = common_limits(p);
     if (!limit && p.page_size < 1) limit = "pages of at least one token";
-    if (!limit && ((long long)p.pages * p.page_size >= 0x7FFFFFFFll || (long long)p.table_width * p.page_size >= 0x7FFFFFFFll - 65536))
-        limit = "fewer than 2^31 tokens in the cache and in one row of the page table";
+    if (!limit && ((long long)p.pages * p.page_size >= 0x7FFFFFFFll || (long long)p.table_width * p.page_size >= 0x40000000ll))
+        limit = "fewer than 2^31 tokens in the cache and 2^30 in one row of the page table";
     if (!limit && p.heads < 1) limit = "at least one head";
     if (limit) return call_fail(name, TOPS_ERR_UNSUPPORTED, limit, outs);
     if (!on_current_device({c.q, c.key_cache, c.value_cache, c.page_table, c.query_start, c.kv_length, y}))
@@ -145,7 +145,7 @@ TOPS_API int tops_paged_attention_forward(const PagedAttentionCall* call) {
     p.query_start = reinterpret_cast<const int*>(c.query_start->data);
     p.kv_length = reinterpret_cast<const int*>(c.kv_length->data);
     p.scale_log2 = c.scale * kLog2E;
-    p.window = c.window;
+    p.window = c.window < p.keys ? c.window : 0;             // a window that no sequence can outgrow is none
     p.dtype = c.q->dtype;
     p.status = device_status_word();
     if (!run_attention(p)) return tops_last_error();
@@ -189,7 +189,7 @@ TOPS_API int tops_cross_attention_forward(const CrossAttentionCall* call) {
     }
     const char* limit = common_limits(p);
     if (!limit && p.heads < 1) limit = "at least one head";
-    if (!limit && p.keys >= 0x7FFFFFFF - 65536) limit = "fewer than 2^31 keys";
+    if (!limit && p.keys >= 0x40000000) limit = "fewer than 2^30 keys";
     if (limit) return call_fail(name, TOPS_ERR_UNSUPPORTED, limit, outs);
     for (const Tensor* t : {c.q, c.k, c.v, c.key_length, c.mask})
         if (overlap(t, y)) return call_fail(name, TOPS_ERR_INVALID, "y shares memory with an operand", outs);

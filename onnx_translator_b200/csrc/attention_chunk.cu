@@ -13,6 +13,11 @@
 // As in the kernel for few rows the work is split evenly: all items -- (two row tiles, key head) with their keys -- stand in one row, weighted by the keys
 // they see, and each of the 148 blocks takes an equal piece of it; pieces of items are joined by a second kernel.
 //
+// Measured (bf16, dim 128, 32 heads over 8 key heads): 2048 tokens over 32768 keys before them 1010 us, 1.12 PFLOP/s (0.67 of a cuBLAS burst), 1213 us when the card is at
+// its power limit (0.93 PFLOP/s; cuBLAS 1.38 there); a prompt of 8192 tokens 500 us, 1.10 PFLOP/s.  A pair of tiles takes about 3450 cycles: a tile's softmax (2050:
+// exponentials 1300, maximum 400, tensor memory and barriers 350) and its two products (1024, and more while both tiles compete) follow one another, and the other tile fills
+// the gaps.  Tried and not kept: a quarter of the exponentials as a polynomial on the multiply-add units (1066 us), the product begun on the first 96 keys' weights (1040 us).
+//
 // Warps 0-3 and 4-7 softmax of the two tiles, warp 8 copies keys and values (TMA, page by page), warp 9 issues the MMAs, warp 10 finds the next item and
 // copies its queries.
 #include "attention_join.cuh"
@@ -64,10 +69,10 @@ __device__ __forceinline__ ChunkSequence chunk_sequence(const AttentionProblem& 
 }
 __device__ __forceinline__ long long weight_of_first(const ChunkSequence& w, long long n) { return n * w.base + (long long)w.slope * (n * (n + 1) / 2); }
 
-__device__ __forceinline__ long long chunk_total(const AttentionProblem& p, int item_tokens) {
+__device__ __forceinline__ long long chunk_total(const AttentionProblem& p, int item_tokens, const ChunkSequence& head) {     // head: the lane's own of the first 32, fetched before
     long long sum = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
-        const ChunkSequence w = chunk_sequence(p, b, item_tokens);
+        const ChunkSequence w = b < 32 ? head : chunk_sequence(p, b, item_tokens);
         sum += weight_of_first(w, w.count);
     }
     #pragma unroll
@@ -77,12 +82,12 @@ __device__ __forceinline__ long long chunk_total(const AttentionProblem& p, int 
 
 struct ChunkPlace { ChunkSequence w; int seq, item, kv_head; long long offset, weight; };
 
-__device__ __forceinline__ ChunkPlace chunk_place(const AttentionProblem& p, long long x, int item_tokens) {
+__device__ __forceinline__ ChunkPlace chunk_place(const AttentionProblem& p, long long x, int item_tokens, const ChunkSequence& head) {
     const int lane = threadIdx.x & 31;
     ChunkPlace at = {};
     long long before = 0;
     for (int base = 0; base < p.batch; base += 32) {
-        const ChunkSequence w = chunk_sequence(p, base + lane, item_tokens);
+        const ChunkSequence w = base == 0 ? head : chunk_sequence(p, base + lane, item_tokens);
         const long long mine = weight_of_first(w, w.count) * p.kv_heads;
         long long sum = mine;
         #pragma unroll
@@ -186,6 +191,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     if (warp == 8 && lane == 0) { umma::tma_prefetch_desc(&k_map); umma::tma_prefetch_desc(&v_map); umma::tma_prefetch_desc(&q_map); }
     asm volatile("griddepcontrol.wait;" ::: "memory");         // nothing so far has touched global or tensor memory
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    ChunkSequence head = {0, 0, 0, 0, 0, 0};
+    if (warp == 10) head = chunk_sequence(p, lane, item_tokens);
     if (warp == 9) umma::tmem_alloc(&tmem_slot, 512);
     umma::fence_before_sync();
     __syncthreads();
@@ -198,7 +205,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == 10) {
             // ---- items and their queries ------------------------------------------------------------------------------------
-            const long long total = chunk_total(p, item_tokens);
+            const long long total = chunk_total(p, item_tokens, head);
             const long long share = (total + gridDim.x - 1) / gridDim.x;
             const long long x0 = min((long long)blockIdx.x * share, total), x1 = min(x0 + share, total);
             long long x = x0;
@@ -210,7 +217,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 seg.n = -1;
                 int page = 0, item_first = 0;
                 if (x < x1) {
-                    const ChunkPlace at = chunk_place(p, x, item_tokens);
+                    const ChunkPlace at = chunk_place(p, x, item_tokens, head);
                     seg.t = chunk_rows(p, at, item_tokens);
                     item_first = at.item * item_tokens;
                     seg.kv_head = at.kv_head;

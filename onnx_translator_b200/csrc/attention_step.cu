@@ -17,11 +17,15 @@
 // it, possibly the end of one item, some whole items and the beginning of another.  The pipeline runs on across items.  An item that lies inside one share
 // is stored at once; of an item that spans several, each block leaves (m, l, o) in scratch memory, at most two per block, and a
 // second small kernel joins them in the order of the keys.  (Clusters that join through distributed shared memory were measured first: the GPU
-// holds only 15 clusters of eight such blocks at a time, 120 of 148 SMs, and 16 items then took two rounds: 235 us where this takes REPLACE_LONG.)
+// holds only 15 clusters of eight such blocks at a time, 120 of 148 SMs, and 16 items then took two rounds: 235 us where this takes 151.)
 //
 // Warps 0-3 and 8-11: two softmax groups that take the items in turn -- one finishes its item (sums, tensor memory, stores) while the other
 // is in the next item's tiles.  Warp 4 copies (TMA, page by page, 128 keys of K or V per ring slot), warp 5 issues the MMAs, warp 6 finds the next
 // item and brings its queries.
+//
+// Measured (dim 128, 32 heads over 8 key heads): one new token for 64 sequences of 300 to 8192 keys 127 us, 6.1 TB/s; for two of 131072 and 100003 keys 151 us, 6.4 TB/s (a
+// plain copy: 6.57); for one of 511 keys 10 us, a chain of latencies: finding the item, four tiles of 0.9 us, the result.  A tile costs the MMA warp about 1650 cycles
+// (sixteen instructions of 39 and the barriers between), copying it 2600.
 #include "attention_join.cuh"
 
 #include <type_traits>
@@ -73,11 +77,11 @@ template <int N> __device__ __forceinline__ SequenceWork sequence_work(const Att
 // Where a unit of that row lies: row tile, key head and unit inside them.
 struct UnitPlace { SequenceWork w; int seq, row_tile, kv_head, unit; };
 
-// All units; called by whole warps.
-template <int N> __device__ __forceinline__ int total_units(const AttentionProblem& p, bool whole) {
+// All units; called by whole warps.  `head` is the lane's own of the first 32 sequences, fetched before.
+template <int N> __device__ __forceinline__ int total_units(const AttentionProblem& p, bool whole, const SequenceWork& head) {
     int sum = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
-        const SequenceWork w = sequence_work<N>(p, b, whole);
+        const SequenceWork w = b < 32 ? head : sequence_work<N>(p, b, whole);
         sum += w.row_tiles * w.units;
     }
     #pragma unroll
@@ -85,12 +89,12 @@ template <int N> __device__ __forceinline__ int total_units(const AttentionProbl
     return sum * p.kv_heads;
 }
 
-template <int N> __device__ __forceinline__ UnitPlace place_unit(const AttentionProblem& p, int x, bool whole) {
+template <int N> __device__ __forceinline__ UnitPlace place_unit(const AttentionProblem& p, int x, bool whole, const SequenceWork& head) {
     const int lane = threadIdx.x & 31;
     UnitPlace at = {};
     int before = 0;
     for (int base = 0; base < p.batch; base += 32) {
-        const SequenceWork w = sequence_work<N>(p, base + lane, whole);
+        const SequenceWork w = base == 0 ? head : sequence_work<N>(p, base + lane, whole);
         const int mine = w.row_tiles * w.units * p.kv_heads;
         int sum = mine;
         #pragma unroll
@@ -222,6 +226,9 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     // waits for this grid before it reads.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const bool whole = parts.o == nullptr;                     // the unit is the item: nothing is split, nothing joined
+    SequenceWork head = {0, 0, 0, 0, 0};
+    if (warp == 6) head = sequence_work<R>(p, lane, whole);
     if (warp == 5) umma::tmem_alloc(&tmem_slot, L::kColumns);
     umma::fence_before_sync();
     __syncthreads();
@@ -231,8 +238,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
 
     if (warp == 6) {
         // ---- items: what this block works on, and its queries ---------------------------------------------------------------
-        const bool whole = parts.o == nullptr;                 // the unit is the item: nothing is split, nothing joined
-        const int total = total_units<R>(p, whole);
+        const int total = total_units<R>(p, whole, head);
         const int share = (total + (int)gridDim.x - 1) / (int)gridDim.x;
         const int x0 = min((int)blockIdx.x * share, total), x1 = min(x0 + share, total);
         int x = x0, s = 0;
@@ -244,7 +250,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             seg.n = -1;
             int page = 0;
             if (x < x1) {
-                at = place_unit<R>(p, x, whole);
+                at = place_unit<R>(p, x, whole, head);
                 seg.t = row_tile_of<R>(p, at);
                 seg.kv_head = at.kv_head;
                 const int take = min(at.w.units - at.unit, x1 - x), first = first_tile_of(p, at);
