@@ -418,8 +418,10 @@ int tops_dynamic_quantize_apply(const Tensor* x, const Tensor* range, Tensor* y,
    call), sums and softmax statistics are float32, every result is rounded once.  Tensors are dense; a cache is
    [pages, page_size, kv_heads, dim].  Index tensors live in device memory and are not read by the host: an index that
    points outside its table is never followed -- the row it belongs to is zero-filled (or, for a page, reads as zero keys and values; for
-   a slot, is not stored) and the next tops_sync or download reports TOPS_ERR_INVALID.  No call allocates device memory or
-   keeps state, so captured sequences and other streams may run the same operators at the same time.
+   a slot, is not stored) and the next tops_sync or download reports TOPS_ERR_INVALID.  Scratch (partial results of sequences
+   that several SMs share) is taken from the stream-ordered pool and returned within the call; no state is kept, so captured
+   sequences and other streams may run the same operators at the same time.  All tensors of a call have to belong to the
+   current device.
    Return TOPS_OK or the recorded error; a rejected call zero-fills its outputs and leaves caches and operands that an output shares memory with as they
    were. */
 
@@ -455,8 +457,9 @@ int tops_qk_norm_rotary_forward(const QKNormRotaryCall* call);
    included: the i-th of n new tokens stands at position p = kv_length[b] - n + i and sees the keys j <= p, with a window
    also only j > p - window.  A token that sees no key (p < 0) gets zeros; rows of y in front of query_start[0] and behind
    query_start[B] are left as they are.  One new token per sequence and whole prompts are both served; float16 / bfloat16 heads of
-   up to 256 (a multiple of 8) run on tensor cores, the rest in float32 arithmetic.  Keys and values behind kv_length may hold
-   anything.  The tables have to be consistent: 0 <= query_start[b] <= query_start[b + 1] <= rows of q (rows outside are not
+   up to 256 (a multiple of 8, 16-byte aligned) run on tensor cores, fastest with pages that are a multiple of 8 and divide 128, or
+   are a multiple of 128; the rest runs in float32 arithmetic.  Keys and values behind kv_length may hold
+   anything; a NaN or infinity in a key or value that some row sees may reach every row that shares its 128 keys.  The tables have to be consistent: 0 <= query_start[b] <= query_start[b + 1] <= rows of q (rows outside are not
    touched), kv_length[b] <= table width * page_size (more is cut to that). */
 typedef struct PagedAttentionCall {
     const Tensor* q;            /* [T, H, D] */

@@ -37,7 +37,7 @@ def test_paged(dtype, shape, batch):
     assert_close(run_paged(problem), want, tol, batch)
 
 
-@pytest.mark.parametrize("window", [1, 5, 16, 100, 4096])
+@pytest.mark.parametrize("window", [1, 5, 16, 100, 4096, 2 ** 31 - 1])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [64, 128])
 def test_paged_window(dtype, window, dim):
