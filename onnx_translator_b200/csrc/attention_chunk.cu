@@ -612,7 +612,7 @@ template <typename T, int DB, int SLOTS> static bool launch_chunk(const Attentio
     const bool masked = p.mask_kind != kMaskNone;
     const void* kernel = masked ? (const void*)attention_chunk_kernel<T, DB, SLOTS, true> : (const void*)attention_chunk_kernel<T, DB, SLOTS, false>;
     if (!ensure_dynamic_smem(kernel, L::kSmem)) return false;
-    const long long items = attention_tiles(p, 2 * tile_tokens * p.group) * p.kv_heads, most = items * ((p.keys + kChunkKeys - 1) / kChunkKeys);
+    const long long items = attention_tiles(p, 2 * tile_tokens * p.group) * p.kv_heads, most = items * (p.keys > 0 ? (p.keys + kChunkKeys - 1) / kChunkKeys : 1);
     const int blocks = (int)(most < (long long)st->sm_count ? most : (long long)st->sm_count);
     cudaStream_t stream = current_stream();
     PartialResults parts;
@@ -627,7 +627,7 @@ template <typename T, int DB, int SLOTS> static bool launch_chunk(const Attentio
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = overlap_launches();
     void* args[] = {&q_map, &k_map, &v_map, &copy, &box_rows, &tile_tokens, &parts};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_chunk");
     ok = join_partials<T, kChunkRows, L::kDims>(copy, parts, blocks, stream, ok);

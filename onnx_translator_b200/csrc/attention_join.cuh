@@ -7,6 +7,8 @@
 
 #include "attention_common.cuh"
 
+#include <cstdlib>
+
 namespace tops {
 
 struct JoinJob {
@@ -21,6 +23,12 @@ struct PartialResults {          // scratch of one call, from the stream-ordered
     float2* stats = nullptr;     // [2 * blocks][N]: maximum, sum of weights
     JoinJob* jobs = nullptr;     // [blocks]
 };
+
+// One launch attribute (a kernel is scheduled while its predecessor drains), or none with TOPS_PDL=0.
+inline unsigned overlap_launches() {
+    static const unsigned on = [] { const char* e = getenv("TOPS_PDL"); return e && e[0] == '0' ? 0u : 1u; }();
+    return on;
+}
 
 inline bool allocate_partials(PartialResults& parts, int blocks, int rows, int dims, cudaStream_t stream) {
     const size_t o_bytes = (size_t)2 * blocks * rows * dims * sizeof(float), stat_bytes = (size_t)2 * blocks * rows * sizeof(float2);
@@ -143,12 +151,12 @@ bool join_partials(const AttentionProblem& p, const PartialResults& parts, int b
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cudaLaunchConfig_t cfg = {};
-        constexpr int ROWS = N >= 64 ? 32 : 4;
+        constexpr int ROWS = N >= 64 ? 8 : 4;
         cfg.gridDim = dim3((unsigned)blocks, N / ROWS);
         cfg.blockDim = dim3(kJoinThreads);
         cfg.stream = stream;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = overlap_launches();
         AttentionProblem copy = p;
         PartialResults copy_parts = parts;
         void* args[] = {&copy, &copy_parts};

@@ -672,7 +672,7 @@ template <typename T, int DB, int R, int SLOTS> static bool launch_step(const At
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = overlap_launches();
     void* args[] = {&k_map, &v_map, &copy, &box_rows, &parts};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_step");
     if (!whole) ok = join_partials<T, R, L::kDims>(copy, parts, blocks, stream, ok);

@@ -167,6 +167,25 @@ def test_a_page_outside_the_cache_is_not_followed(dtype, tokens):
         capi.check(lib)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 150])
+def test_a_page_table_without_columns(dtype, tokens):
+    """No sequence can have a key: zeros for the sequences' rows, nothing else is touched; a length is cut and reported."""
+    from onnx_translator_b200 import capi
+    lib = capi.load()
+    for length, status in ((0, 0), (5, 1)):
+        problem = Paged(_rng(dtype, "no columns"), dtype, 4, 2, 64, 16, [(tokens, 0)], extra_rows=2)
+        problem.table = np.zeros((1, 0), np.int32)
+        problem.kv_length[:] = length
+        call = problem.call()
+        lib.tops_clear_error()
+        assert lib.tops_paged_attention_forward(ctypes.byref(call)) == 0, lib.tops_last_error_message()
+        assert lib.tops_sync() == status
+        lib.tops_clear_error()
+        got = to_f64(call.kept["y"].numpy(), dtype)
+        assert np.all(got[:tokens] == 0.0) and np.all(got[tokens:] == 7.0)
+
+
 def test_inconsistent_tables_stay_in_bounds():
     """Sequence bounds past the rows of q and lengths past the table are cut and reported."""
     from onnx_translator_b200 import capi
