@@ -630,7 +630,7 @@ template <typename T, int DB, int SLOTS> static bool launch_chunk(const Attentio
     cfg.numAttrs = overlap_launches();
     void* args[] = {&q_map, &k_map, &v_map, &copy, &box_rows, &tile_tokens, &parts};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_chunk");
-    ok = join_partials<T, kChunkRows, L::kDims>(copy, parts, blocks, stream, ok);
+    ok = join_partials<T, kChunkRows, L::kDims>(copy, parts, blocks, items, stream, ok);
     if (ok) count_tensor_core_launch();
     return ok;
 }

@@ -40,18 +40,18 @@ inline bool allocate_partials(PartialResults& parts, int blocks, int rows, int d
     return true;
 }
 
-// Block (c, q): ROWS rows of job c, eight warps.  With few parts a warp joins whole rows by itself, all loads in flight together; with many (a few long sequences
+// Block (c, q): `rows` rows of job c, eight warps.  With few parts a warp joins whole rows by itself, all loads in flight together; with many (a few long sequences
 // over all SMs) the warps take every eighth part of a row and meet in shared memory.
 constexpr int kJoinThreads = 256;
-template <typename T, int N, int DIMS, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttentionProblem p, const PartialResults parts) {
+template <typename T, int N, int DIMS>
+__global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_constant__ AttentionProblem p, const PartialResults parts, const int rows) {
     constexpr int WARPS = kJoinThreads / 32, QUADS = DIMS / 4, PER_LANE = (QUADS + 31) / 32;
     __shared__ float4 partial[WARPS][QUADS];
     __shared__ float partial_l[WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const JoinJob job = parts.jobs[blockIdx.x];
-    const int row_begin = (int)blockIdx.y * ROWS, row_end = min(row_begin + ROWS, job.t.rows);
+    const int row_begin = (int)blockIdx.y * rows, row_end = min(row_begin + rows, job.t.rows);
     if (job.parts == 0 || row_begin >= row_end) return;
     auto slot = [&](int k) { return k == 0 ? job.slot : 2 * ((int)blockIdx.x + k); };
     const bool aligned = (p.dim & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(T) - 1)) == 0;
@@ -143,24 +143,26 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join(const __grid_cons
     }
 }
 
-// Enqueues the join (when the main kernel was launched: `ok`) and gives the scratch back in stream order.
+// Enqueues the join (when the main kernel was launched: `ok`) and gives the scratch back in stream order.  `items` (an upper bound) tells how many parts an item has about: with
+// many, rows are the longer work and are spread over more blocks (256 rows, 18 parts each: 83 us with 32 rows a block, 44 with 8); with few, blocks without work
+// cost more (13 ragged windows: 47 against 50 us).
 template <typename T, int N, int DIMS>
-bool join_partials(const AttentionProblem& p, const PartialResults& parts, int blocks, cudaStream_t stream, bool ok) {
+bool join_partials(const AttentionProblem& p, const PartialResults& parts, int blocks, long long items, cudaStream_t stream, bool ok) {
     if (ok) {
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cudaLaunchConfig_t cfg = {};
-        constexpr int ROWS = N >= 64 ? 8 : 4;
-        cfg.gridDim = dim3((unsigned)blocks, N / ROWS);
+        int rows = N < 64 ? 4 : blocks >= 6 * items ? 8 : 32;
+        cfg.gridDim = dim3((unsigned)blocks, (unsigned)(N / rows));
         cfg.blockDim = dim3(kJoinThreads);
         cfg.stream = stream;
         cfg.attrs = attr;
         cfg.numAttrs = overlap_launches();
         AttentionProblem copy = p;
         PartialResults copy_parts = parts;
-        void* args[] = {&copy, &copy_parts};
-        ok = check_cuda(cudaLaunchKernelExC(&cfg, (const void*)attention_join<T, N, DIMS, ROWS>, args), "attention_join");
+        void* args[] = {&copy, &copy_parts, &rows};
+        ok = check_cuda(cudaLaunchKernelExC(&cfg, (const void*)attention_join<T, N, DIMS>, args), "attention_join");
     }
     return TOPS_CUDA_OK(cudaFreeAsync(parts.o, stream)) && ok;
 }

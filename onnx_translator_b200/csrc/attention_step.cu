@@ -675,7 +675,7 @@ template <typename T, int DB, int R, int SLOTS> static bool launch_step(const At
     cfg.numAttrs = overlap_launches();
     void* args[] = {&k_map, &v_map, &copy, &box_rows, &parts};
     bool ok = check_cuda(cudaLaunchKernelExC(&cfg, kernel, args), "attention_step");
-    if (!whole) ok = join_partials<T, R, L::kDims>(copy, parts, blocks, stream, ok);
+    if (!whole) ok = join_partials<T, R, L::kDims>(copy, parts, blocks, items, stream, ok);
     if (ok) count_tensor_core_launch();
     return ok;
 }
