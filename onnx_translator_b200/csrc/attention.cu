@@ -64,15 +64,15 @@ bool make_cache_map(CUtensorMap* map, const AttentionProblem& p, const void* bas
     return make_tensor_map(map, base, 2, false, p.dtype == DTYPE_FLOAT16, 4, dims, strides, box, nullptr);
 }
 
-// The kernel, by the rows of a sequence (tokens times heads per key head, on average: the host does not know each length).  Measured, 8 sequences of 4000 keys, 8 key
-// heads, us, few-rows kernel / many-rows kernel: dim 128, 16 rows 39 / 44, 32 rows 62 / 47 (one sequence of 16000 keys: 45 / 80), 48 rows 152 / 46; dim 64, 16 rows
-// 30 / 37, 32 rows 80 / 40.  Heads above 128 and scales that are not positive stay with the few-rows kernel (dim 256, 64 rows: 135, mma.sync kernel 409), pages that no
-// copy box fits go to the mma.sync kernel.
+// The kernel, by the rows of a sequence (tokens times heads per key head, on average: the host does not know each length).  Measured, us, few-rows kernel / many-rows
+// kernel, 8 sequences of 4000 keys and 8 key heads: dim 128, 16 rows 39 / 43, 20 rows 52 / 44, 32 rows 62 / 47; dim 64, 16 rows 30 / 37.  One sequence of 16000 keys, dim 128:
+// 16 rows 31 / 37, 20 rows 40 / 37, 32 rows 45 / 38.  Heads above 128 and scales that are not positive stay with the few-rows kernel (dim 256, 64 rows: 135, mma.sync
+// kernel 409); pages that no copy box fits go to the mma.sync kernel.
 static bool run_attention(const AttentionProblem& p) {
     if (!whole_pieces(p)) return attention_fma(p);
     if (cache_box_rows(p) > 0) {
         const long long rows = (long long)p.queries * p.group / (p.page_table ? p.batch : 1);
-        const bool few = rows <= (p.dim <= 64 ? 16 : 32);
+        const bool few = rows <= 16;
         if (attention_step_fits(p) && (few || !attention_chunk_takes(p))) return attention_step(p);
         if (attention_chunk_takes(p)) return attention_chunk(p);
     }
