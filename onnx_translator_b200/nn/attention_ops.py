@@ -92,7 +92,8 @@ class QKNormRotary(_StructCall):
 class PagedAttention(_StructCall):
     """A ragged batch of new tokens attends, causally, over a paged cache that holds their keys and values already.
 
-    inputs: [q, key_cache, value_cache, page_table, query_start, kv_length]; ``scale`` None is 1 / sqrt(dim)."""
+    inputs: [q, key_cache, value_cache, page_table, query_start, kv_length]; ``scale`` None is 1 / sqrt(dim).  Rows of the result that
+    belong to no sequence are zeros; in a recorded plan, which reuses its tensors, they keep what the last run that owned them left."""
 
     def __init__(self, inputs, outputs, scale=None, window=0, dtype="bfloat16", version="17"):
         super().__init__(inputs, outputs)
