@@ -376,19 +376,22 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         auto step = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1u; } };
         int s = -1, left = 0, tile = 0;                        // segment, tiles of it whose scores are still to come, number of the next tile
         bool ok = true, fresh = false;
-        // advances to the next tile and issues its scores; false at the end (or when the block gives up: ok false)
-        auto scores = [&] {
+        // Advances to the next tile, no further than segment `limit`, and issues its scores.  The segment behind an empty one is only published when the one before
+        // has been stored, so with a tile's product still to issue the look ahead ends at the next segment.
+        enum { kEnd, kIssued, kLater };
+        auto scores = [&](int limit) {
             fresh = false;
             while (left == 0) {
+                if (s >= limit) return kLater;
                 s++;
-                if (!wait(&seg_full[s & 1], (uint32_t)(s >> 1) & 1u)) { ok = false; return false; }
+                if (!wait(&seg_full[s & 1], (uint32_t)(s >> 1) & 1u)) { ok = false; return kEnd; }
                 left = segments[s & 1].n;
                 __syncwarp();
-                if (left < 0) return false;
+                if (left < 0) return kEnd;
                 fresh = true;
                 if (left == 0 && lane == 0) umma::mbar_arrive(&seg_empty[s & 1]);
             }
-            if (!wait(&full[slot], phase)) { ok = false; return false; }
+            if (!wait(&full[slot], phase)) { ok = false; return kEnd; }
             umma::fence_after_sync();
             left--;
             const uint64_t da = umma::smem_desc_k_major_sw128(ring + slot * L::kSlotBytes), db = umma::smem_desc_k_major_sw128(q_tiles + (s & 1) * L::kQBytes);
@@ -404,10 +407,11 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             __syncwarp();
             tile++;
             step();                                            // on to this tile's values
-            return true;
+            return kIssued;
         };
-        bool more = scores();
-        while (more && ok) {
+        constexpr int kNoLimit = 0x7FFFFFFF;
+        int more = scores(kNoLimit);
+        while (more == kIssued && ok) {
             const int i = tile - 1;
             const bool first = fresh;
             const uint32_t o_at = tmem_o + (uint32_t)((s & 1) * L::kOAccs * N);
@@ -415,7 +419,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
             const bool last = left == 0;
             const uint32_t v_slot = slot, v_phase = phase;
             step();
-            more = scores();
+            more = scores(of + 1);
             if (!ok) break;
             ok = wait(&p_ready[i & 1], (uint32_t)(i >> 1) & 1u) && wait(&full[v_slot], v_phase);
             if (!ok) break;
@@ -433,6 +437,7 @@ attention_step_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
                 if (last) umma::mma_commit(&o_full[of & 1]);   // a barrier of its own: the other group's tiles may be far ahead when this one is looked at
             }
             __syncwarp();
+            if (more == kLater) more = scores(kNoLimit);
         }
         if (!ok) {
             if (umma::elect_one()) umma::mma_commit(&drained);

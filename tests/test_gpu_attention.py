@@ -387,3 +387,100 @@ def test_unaligned_operands():
         for _, handle in moved.values():
             lib.free_tensor(handle)
         capi.check(lib)
+
+
+@pytest.mark.parametrize("dtype,page,tokens", [("bfloat16", 64, 1), ("bfloat16", 64, 200), ("bfloat16", 40, 1), ("float16", 16, 12), ("float32", 64, 2)])
+def test_offsets_past_32_bits(dtype, page, tokens):
+    """Pages whose elements lie more than 2^31 from the start of the cache, filled by the append and read by attention."""
+    import torch
+    from onnx_translator_b200 import capi
+    lib = capi.load()
+    torch_type = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32}[dtype]
+    heads, kv_heads, dim, keys = 16, 8, 128, 300
+    pages = (2 ** 31 // (kv_heads * dim)) // page + 40
+    rng = _rng("far", dtype, page, tokens)
+    q, k, v = exact(rng, (tokens, heads, dim), dtype), exact(rng, (keys, kv_heads, dim), dtype), exact(rng, (keys, kv_heads, dim), dtype)
+    caches = [torch.zeros((pages, page, kv_heads, dim), dtype=torch_type, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    shape, nd = capi.shape_array(caches[0].shape)
+    handles = [lib.tops_wrap(c.data_ptr(), shape, nd, capi.DTYPE_MAP[dtype]) for c in caches]
+    table = (pages - 1 - np.arange(-(-keys // page))).astype(np.int32)[None]
+    j = np.arange(keys)
+    slots = table[0, j // page].astype(np.int64) * page + j % page
+    append = fill(capi.CQKNormRotaryCall(), q=device(np.zeros((keys, heads, dim)), dtype), k=device(k, dtype), v=device(v, dtype),
+                  q_out=device(np.zeros((keys, heads, dim)), dtype), slots=device(slots.astype(np.int32), "int32"))
+    call = fill(capi.CPagedAttentionCall(scale=dim ** -0.5), q=device(q, dtype), page_table=device(table, "int32"),
+                query_start=device(np.array([0, tokens], np.int32), "int32"), kv_length=device(np.array([keys], np.int32), "int32"),
+                y=device(np.full(q.shape, 7.0), dtype))
+    for c in (append, call):
+        c.key_cache, c.value_cache = (ctypes.cast(h, ctypes.c_void_p) for h in handles)
+    assert lib.tops_qk_norm_rotary_forward(ctypes.byref(append)) == 0, lib.tops_last_error_message()
+    assert lib.tops_paged_attention_forward(ctypes.byref(call)) == 0, lib.tops_last_error_message()
+    seen = j[None, :] <= (keys - tokens + np.arange(tokens))[:, None]
+    want, tol = attention(q, k, v, seen, dim ** -0.5, dtype)
+    got = to_f64(call.kept["y"].numpy(), dtype)
+    capi.check(lib)
+    assert_close(got, want, tol)
+    for h in handles:
+        lib.free_tensor(h)
+    del caches
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cross_attention_on_another_stream_and_captured(dtype):
+    """The caller's stream carries the call; one captured call serves new contents and lengths."""
+    import torch
+    from onnx_translator_b200 import capi
+    lib = capi.load()
+    for queries in (1, 150):
+        rng = _rng("stream", dtype, queries)
+        sets = [(exact(rng, (2, queries, 4, 64), dtype), exact(rng, (2, 700, 2, 64), dtype), exact(rng, (2, 700, 2, 64), dtype),
+                 np.array([n, 700 - n], np.int32)) for n in (650, 33)]
+        call = fill(capi.CCrossAttentionCall(scale=0.125), q=device(sets[0][0], dtype), k=device(sets[0][1], dtype), v=device(sets[0][2], dtype),
+                    key_length=device(sets[0][3], "int32"), y=device(np.full(sets[0][0].shape, 7.0), dtype))
+        others = [device(x, dtype) for x in sets[1][:3]] + [device(sets[1][3], "int32")]
+        lib.tops_sync()
+        stream = torch.cuda.Stream()
+        lib.tops_set_stream(stream.cuda_stream)
+        try:
+            assert lib.tops_capture_begin() == 0
+            assert lib.tops_cross_attention_forward(ctypes.byref(call)) == 0
+            graph = lib.tops_capture_end()
+            for which in (0, 1):
+                if which:
+                    for name, other in zip(("q", "k", "v", "key_length"), others):
+                        lib.flatten_forward(other.handle, call.kept[name].handle)
+                assert lib.tops_capture_launch(graph) == 0
+                got = to_f64(call.kept["y"].numpy(), dtype)
+                q, k, v, lengths = sets[which]
+                for b in range(2):
+                    want, tol = attention(q[b], k[b], v[b], np.broadcast_to(np.arange(700) < lengths[b], (queries, 700)), 0.125, dtype)
+                    assert_close(got[b], want, tol)
+            lib.tops_capture_free(graph)
+        finally:
+            lib.tops_set_stream(None)
+        capi.check(lib)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("most", [1, 2, 30])
+def test_hundreds_of_short_sequences(dtype, most):
+    """More sequences than lanes and than SMs, many of them without keys or without tokens: every block goes through dozens of items."""
+    rng = _rng("hundreds", dtype, most)
+    pairs = []
+    for b in range(333):
+        n = int(rng.integers(0, most + 1)) if most > 1 else 1
+        pairs.append((n, 0 if b % 7 == 3 else n + int(rng.integers(0, 200 if b % 5 else 700))))
+    problem = Paged(rng, dtype, 8, 2, 64, 16, pairs, extra_rows=3)
+    want, tol = problem.want()
+    got = run_paged(problem)
+    assert_close(got[:len(want)], want, tol)
+    assert np.all(got[len(want):] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [1, 100])
+def test_hundreds_of_short_sources(dtype, queries):
+    rng = _rng("sources", dtype, queries)
+    _cross(dtype, 101, queries, 150, 4, 2, 64, lengths=rng.integers(0, 151, 101), mask=(rng.random((101, 150)) < 0.8).astype(np.uint8))
